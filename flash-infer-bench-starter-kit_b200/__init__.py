@@ -4,6 +4,8 @@ Public surface:
   kernel(...)            drop-in for the reference solution's entry point
   inputs.make_inputs     seeded synthetic inputs with the definition's shapes
   ep.EPMoE               expert-parallel layer over NCCL (one process per GPU)
+  sort_tokens, dispatch, combine
+                         tokens sorted by expert and back, with gradients
 
 The directory name is not a Python identifier; load the package with
 ``__graft_entry__.load_package()``, which registers it as ``fib_b200``.
@@ -11,3 +13,4 @@ The directory name is not a Python identifier; load the package with
 
 from .kernel import kernel  # noqa: F401
 from . import inputs  # noqa: F401
+from .tokens import TokenOrder, combine, dispatch, sort_tokens  # noqa: F401

@@ -13,6 +13,9 @@ import threading
 
 LIB_PATH = pathlib.Path(__file__).resolve().parent / "libmoe_fp8_ds.so"
 
+# Element types (enum moe_dtype).
+MOE_F32, MOE_F16, MOE_BF16 = 0, 1, 2
+
 # Status codes (enum moe_status).
 MOE_OK = 0
 MOE_ERR_INVALID_ARGUMENT = 1
@@ -64,6 +67,7 @@ EXPORTS = (
     "moe_fp8_ds_ep_plan_capacity", "moe_fp8_ds_ep_pack_capacity",
     "moe_fp8_ds_selftest_wait_timeout", "moe_fp8_ds_noalloc_read_device_error",
     "moe_fp8_ds_last_cuda_error_string",
+    "moe_tokens_sort", "moe_tokens_dispatch", "moe_tokens_combine", "moe_tokens_combine_backward",
 )
 
 _lib = None
@@ -110,6 +114,10 @@ def load() -> ctypes.CDLL:
         lib.moe_fp8_ds_ep_plan_capacity.argtypes = [P, I32, I32, I32, I32, P, P, P, P]
         lib.moe_fp8_ds_ep_pack_capacity.argtypes = [P, P, P, P, I32, P, I32, I32, I32, P, P]
         lib.moe_fp8_ds_selftest_wait_timeout.argtypes = [P, P]
+        lib.moe_tokens_sort.argtypes = [P, I32, I32, I32, I32, P, P, P, P]
+        lib.moe_tokens_dispatch.argtypes = [P, P, I32, I32, I32, I32, P, P]
+        lib.moe_tokens_combine.argtypes = [P, P, P, I32, I32, I32, I32, I32, P, P]
+        lib.moe_tokens_combine_backward.argtypes = [P, P, P, P, I32, I32, I32, I32, I32, P, P, P]
         for name in EXPORTS:
             if name not in ("moe_fp8_ds_status_string", "moe_fp8_ds_last_cuda_error_string"):
                 getattr(lib, name).restype = ctypes.c_int

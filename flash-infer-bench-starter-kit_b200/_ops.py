@@ -1,0 +1,44 @@
+"""What the operators around the expert products share on the Python side:
+argument checks in the manner of ``kernel(...)`` and the call into the library
+on the tensors' device and its current stream."""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+DTYPES = {torch.float32: _lib.MOE_F32, torch.float16: _lib.MOE_F16, torch.bfloat16: _lib.MOE_BF16}
+
+
+def check_tensor(name, t, dtypes, shape, device):
+    """``shape``: the expected sizes, -1 for any; ``dtypes``: the accepted types; ``device``: None
+    for any CUDA device."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} has dtype {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
+    if t.dim() != len(shape) or any(n != -1 and n != m for n, m in zip(shape, t.shape)):
+        want = ", ".join("any" if n == -1 else str(n) for n in shape)
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected ({want})")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (no CPU path)")
+    if device is not None and t.get_device() != device.index:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def call(name, device, *args):
+    """Run entry point ``name`` with ``args`` (tensors as pointers, None as NULL) on ``device``'s
+    current stream."""
+    fn = getattr(_lib.load(), name)
+    args = [a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args]
+    stream = torch.cuda.current_stream(device.index).cuda_stream
+    if torch.cuda.current_device() == device.index:
+        status = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, stream)
+    if status != _lib.MOE_OK:
+        _lib.check(status, name)

@@ -17,8 +17,9 @@ PKG_DIR = pathlib.Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_NAME = "libmoe_fp8_ds.so"
 LIB_PATH = PKG_DIR / LIB_NAME
-SOURCES = ("api.cu", "route_permute.cu", "gemm_fp8.cu", "gemm_tm.cu", "noalloc.cu", "ep.cu")
-HEADERS = ("common.cuh", "kernels.cuh")
+SOURCES = ("api.cu", "route_permute.cu", "gemm_fp8.cu", "gemm_tm.cu", "noalloc.cu", "ep.cu",
+           "tokens.cu")
+HEADERS = ("common.cuh", "kernels.cuh", "rows.cuh")
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -60,7 +61,7 @@ def build(force: bool = False, verbose: bool = False) -> pathlib.Path:
     """Compile ``libmoe_fp8_ds.so`` (sm_100a) if missing or older than its sources."""
     if not force and not is_stale():
         return LIB_PATH
-    cmd = [_nvcc(), *ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "-shared",
+    cmd = [_nvcc(), "--threads", "0", *ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "-shared",
            "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
            "-o", str(LIB_PATH) + ".tmp", *[str(CSRC / s) for s in SOURCES], "-lcudart"]
     if verbose:

@@ -8,7 +8,7 @@
 #include <mutex>
 #include <string.h>
 
-#include "kernels.cuh"
+#include "rows.cuh"
 
 namespace moe {
 namespace {
@@ -72,6 +72,15 @@ int device_info(DeviceInfo* out) {
 }
 
 }  // namespace
+
+int cuda_status(cudaError_t e) { return e == cudaSuccess ? MOE_OK : cuda_fail(e); }
+
+int require_device(int* sm_count) {
+  DeviceInfo d;
+  const int st = device_info(&d);
+  if (st == MOE_OK && sm_count) *sm_count = d.sm_count;
+  return st;
+}
 
 void* current_cu_context() {
   using CtxGetCurrentFn = CUresult (*)(CUcontext*);

@@ -253,6 +253,52 @@ MOE_API int moe_fp8_ds_ep_unpack(const void* recv, int32_t rows, void* hidden_st
 MOE_API int moe_fp8_ds_ep_combine(const void* partials, const int32_t* slot, int32_t num_tokens, int32_t world,
                                   void* output, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Operators around the expert products (no counterpart in the reference, which
+ * has these steps only inside its fused forward call).  Types are moe_dtype
+ * values; tensors are contiguous and row-major; pointers are aligned to their
+ * element (16-byte alignment gives the widest accesses).  No call keeps state or
+ * needs a workspace.
+ * ------------------------------------------------------------------------- */
+typedef enum moe_dtype {
+  MOE_F32 = 0,
+  MOE_F16 = 1,
+  MOE_BF16 = 2,
+} moe_dtype;
+
+/* Tokens sorted by expert.  topk_ids int32 [T, K]; an id outside
+ * [local_expert_offset, local_expert_offset + E) is not on this shard (so -1
+ * means "no expert").  The T * K pairs (t, k) are ordered by expert, then by
+ * t * K + k; pairs that are not on the shard come last in t * K + k order.
+ * offsets int32 [E + 1] gives each expert's rows, inv_row int32 [T, K] a pair's
+ * row, or -1 - row for a pair that is not on the shard, row_token int32 [T * K]
+ * a row's token, -1 behind the last expert.  E <= 1024, T * K < 2^30.         */
+MOE_API int moe_tokens_sort(const int32_t* topk_ids, int32_t num_tokens, int32_t top_k, int32_t num_local_experts,
+                            int32_t local_expert_offset, int32_t* offsets, int32_t* inv_row, int32_t* row_token,
+                            void* stream);
+
+/* rows[inv_row[t][k]] = hidden[t], rows of pairs that are not on the shard = 0:
+ * hidden [T, width], rows [T * K, width], every row written.                 */
+MOE_API int moe_tokens_dispatch(const void* hidden, const int32_t* inv_row, int32_t num_tokens, int32_t top_k,
+                                int32_t width, int32_t dtype, void* rows, void* stream);
+
+/* out[t] = sum over k of weights[t][k] * rows[inv_row[t][k]] (pairs on the shard
+ * only), summed in fp32 in ascending k and rounded once.  weights fp32 [T, K];
+ * NULL sums without weights, which is the gradient of moe_tokens_dispatch.
+ * out_dtype is rows_dtype, or any type when rows are fp32.                   */
+MOE_API int moe_tokens_combine(const void* rows, const int32_t* inv_row, const float* weights, int32_t num_tokens,
+                               int32_t top_k, int32_t width, int32_t rows_dtype, int32_t out_dtype, void* out,
+                               void* stream);
+
+/* Gradients of moe_tokens_combine from grad_out [T, width] (out_dtype):
+ * grad_rows [T * K, width] (rows_dtype; zero for pairs that are not on the shard)
+ * and grad_weights fp32 [T, K] (zero likewise).  Either may be NULL; rows may be
+ * NULL without grad_weights.                                                 */
+MOE_API int moe_tokens_combine_backward(const void* grad_out, const void* rows, const int32_t* inv_row,
+                                        const float* weights, int32_t num_tokens, int32_t top_k, int32_t width,
+                                        int32_t rows_dtype, int32_t out_dtype, void* grad_rows,
+                                        float* grad_weights, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
