@@ -18,7 +18,7 @@ CSRC = PKG_DIR / "csrc"
 LIB_NAME = "libmoe_fp8_ds.so"
 LIB_PATH = PKG_DIR / LIB_NAME
 SOURCES = ("api.cu", "route_permute.cu", "gemm_fp8.cu", "gemm_tm.cu", "noalloc.cu", "ep.cu",
-           "tokens.cu")
+           "tokens.cu", "swiglu.cu", "w4.cu")
 HEADERS = ("common.cuh", "kernels.cuh", "rows.cuh")
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

@@ -32,6 +32,7 @@ struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Pack {
 };
 
 template <int BYTES> struct Word;
+template <> struct Word<1> { using type = uint8_t; };
 template <> struct Word<2> { using type = uint16_t; };
 template <> struct Word<4> { using type = uint32_t; };
 template <> struct Word<8> { using type = uint2; };

@@ -1,0 +1,304 @@
+// SwiGLU between the two expert products, y = up * gate * sigmoid(gate) for rows
+// x = [up | gate] (the order of W13's halves), with its input kept for the
+// backward pass in 8 bits: every 1x128 block of up and of gate (blocks start at
+// each half's first column, the last may be shorter) becomes e4m3 codes
+//   s = amax / 448 (1 when that is 0),  q = e4m3(x / s),  both in fp32,
+// the layer's activation format.  The backward pass computes from q * s:
+//   grad_up   = g * gate * sig
+//   grad_gate = g * up * sig * (1 + gate * (1 - sig))
+// A block that holds an infinity or a NaN is kept as NaN.
+//
+// Both passes are bound by memory: 2 + 1 elements (forward, nothing kept), 2 + 1
+// elements + 2 bytes (forward), 1 + 2 elements + 2 bytes (backward) for each
+// column, so the kept codes cost the backward pass half of the reads that kept
+// 16-bit inputs would.
+#include "rows.cuh"
+
+namespace moe {
+namespace {
+
+constexpr int kLanes = 16;                       // threads of one 1x128 block
+constexpr int kElems = kBlock / kLanes;          // 8 columns a thread
+constexpr int kThreads = 256;
+constexpr int kRowsAtOnce = kThreads / kLanes;   // rows of a CTA in one step
+
+// sigmoid in fp32.  16-bit outputs keep 11 bits at most, so the short forms
+// (about 2^-21 off) cost them nothing; fp32 outputs get the full ones.
+template <typename T>
+__device__ __forceinline__ float sigmoid(float v) {
+  if constexpr (sizeof(T) == 2) return __fdividef(1.f, 1.f + __expf(-v));
+  return 1.f / (1.f + expf(-v));
+}
+
+// A thread's 8 columns of a block, as 8 / N accesses of N elements: access j
+// covers columns (j * 16 + lane) * N ..., so neighbours read neighbours.
+template <int N>
+__device__ __forceinline__ int column(int j, int lane) { return (j * kLanes + lane) * N; }
+
+template <typename T, int N>
+__device__ __forceinline__ void load_block(const T* p, int lane, int width, float (&v)[kElems]) {
+#pragma unroll
+  for (int j = 0; j < kElems / N; ++j) {
+    const int c = column<N>(j, lane);
+    if (c < width) {                             // width is a multiple of N
+      const Pack<T, N> x = load_stream<T, N>(p + c);
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[j * N + i] = to_float(x.v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[j * N + i] = 0.f;
+    }
+  }
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_block(T* p, int lane, int width, const float (&v)[kElems]) {
+#pragma unroll
+  for (int j = 0; j < kElems / N; ++j) {
+    const int c = column<N>(j, lane);
+    if (c >= width) continue;
+    Pack<T, N> x;
+#pragma unroll
+    for (int i = 0; i < N; ++i) x.v[i] = from_float<T>(v[j * N + i]);
+    store_wide<T, N>(p + c, x);
+  }
+}
+
+// Codes of a block and its scale (the same in all 16 lanes).
+template <int N>
+__device__ __forceinline__ float keep_block(uint8_t* q, int lane, int width, const float (&v)[kElems]) {
+  float amax = 0.f;
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < kElems; ++i) {
+    amax = fmaxf(amax, fabsf(v[i]));             // fmaxf drops NaN: noted apart
+    nan |= v[i] != v[i];
+  }
+  if (nan) amax = INFINITY;
+#pragma unroll
+  for (int off = kLanes / 2; off; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+  float s = __fdiv_rn(amax, kFp8Max);
+  if (s == 0.f) s = 1.f;
+  if (s == INFINITY) s = __int_as_float(0x7fc00000);
+#pragma unroll
+  for (int j = 0; j < kElems / N; ++j) {
+    const int c = column<N>(j, lane);
+    if (c >= width) continue;
+    Pack<uint8_t, N> o;
+    if constexpr (N == 1) {
+      o.v[0] = f32_to_e4m3(__fdiv_rn(v[j], s));
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        const float2 f = make_float2(__fdiv_rn(v[j * N + i], s), __fdiv_rn(v[j * N + i + 1], s));
+        const __nv_fp8x2_storage_t two = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+        o.v[i] = (uint8_t)(two & 0xff);
+        o.v[i + 1] = (uint8_t)(two >> 8);
+      }
+    }
+    if constexpr (N == 1) q[c] = o.v[0];
+    else store_wide<uint8_t, N>(q + c, o);
+  }
+  return s;
+}
+
+template <int N>
+__device__ __forceinline__ void kept_block(const uint8_t* q, int lane, int width, float s, float (&v)[kElems]) {
+#pragma unroll
+  for (int j = 0; j < kElems / N; ++j) {
+    const int c = column<N>(j, lane);
+    Pack<uint8_t, N> o = {};
+    if (c < width) {
+      if constexpr (N == 1) o.v[0] = q[c];
+      else o = load_stream<uint8_t, N>(q + c);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[j * N + i] = e4m3_to_f32(o.v[i]) * s;
+  }
+}
+
+// A CTA takes block `b` of U * 16 rows, so the scales of a block (stored by
+// block, [2 * blocks][R]) are written as whole lines; neighbouring CTAs take
+// neighbouring blocks.  U rows are in flight in each thread.
+template <typename T, int N, int U, bool KEEP>
+__global__ void __launch_bounds__(kThreads)
+swiglu_kernel(const T* __restrict__ x, int R, int I, int blocks, T* __restrict__ y, uint8_t* __restrict__ q,
+              float* __restrict__ scale) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const int tile = (int)blockIdx.x / blocks, b = (int)blockIdx.x - tile * blocks;
+  const int lane = (int)threadIdx.x % kLanes;
+  const int64_t row0 = (int64_t)tile * (U * kRowsAtOnce) + threadIdx.x / kLanes;
+  const int col = b * kBlock, width = I - col < kBlock ? I - col : kBlock;
+  float up[U][kElems], gate[U][kElems];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t r = row0 + u * kRowsAtOnce;
+    const T* p = x + (size_t)r * 2 * I + col;
+    const int w = r < R ? width : 0;
+    load_block<T, N>(p, lane, w, up[u]);
+    load_block<T, N>(p + I, lane, w, gate[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t r = row0 + u * kRowsAtOnce;
+    const int w = r < R ? width : 0;
+    if constexpr (KEEP) {
+      uint8_t* p = q + (size_t)r * 2 * I + col;
+      const float su = keep_block<N>(p, lane, w, up[u]), sg = keep_block<N>(p + I, lane, w, gate[u]);
+      if (lane == 0 && r < R) {
+        scale[(size_t)b * R + r] = su;
+        scale[(size_t)(blocks + b) * R + r] = sg;
+      }
+    }
+    float out[kElems];
+#pragma unroll
+    for (int i = 0; i < kElems; ++i) out[i] = gate[u][i] * sigmoid<T>(gate[u][i]) * up[u][i];
+    store_block<T, N>(y + (size_t)r * I + col, lane, w, out);
+  }
+}
+
+template <typename T, int N, int U>
+__global__ void __launch_bounds__(kThreads)
+swiglu_backward_kernel(const T* __restrict__ g, const uint8_t* __restrict__ q, const float* __restrict__ scale,
+                       int R, int I, int blocks, T* __restrict__ grad_x) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const int tile = (int)blockIdx.x / blocks, b = (int)blockIdx.x - tile * blocks;
+  const int lane = (int)threadIdx.x % kLanes;
+  const int64_t row0 = (int64_t)tile * (U * kRowsAtOnce) + threadIdx.x / kLanes;
+  const int col = b * kBlock, width = I - col < kBlock ? I - col : kBlock;
+  float up[U][kElems], gate[U][kElems], dy[U][kElems];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t r = row0 + u * kRowsAtOnce;
+    const int w = r < R ? width : 0;
+    const float su = r < R ? __ldg(scale + (size_t)b * R + r) : 0.f;
+    const float sg = r < R ? __ldg(scale + (size_t)(blocks + b) * R + r) : 0.f;
+    const uint8_t* p = q + (size_t)r * 2 * I + col;
+    kept_block<N>(p, lane, w, su, up[u]);
+    kept_block<N>(p + I, lane, w, sg, gate[u]);
+    load_block<T, N>(g + (size_t)r * I + col, lane, w, dy[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t r = row0 + u * kRowsAtOnce;
+    const int w = r < R ? width : 0;
+    float du[kElems], dg[kElems];
+#pragma unroll
+    for (int i = 0; i < kElems; ++i) {
+      const float sig = sigmoid<T>(gate[u][i]), gs = dy[u][i] * sig;
+      du[i] = gs * gate[u][i];
+      dg[i] = gs * up[u][i] * (1.f + gate[u][i] * (1.f - sig));
+    }
+    T* p = grad_x + (size_t)r * 2 * I + col;
+    store_block<T, N>(p, lane, w, du);
+    store_block<T, N>(p + I, lane, w, dg);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+struct SwigluGrid {
+  int blocks;
+  int64_t ctas;
+};
+SwigluGrid swiglu_grid(int R, int I, int U) {
+  const int blocks = (I + kBlock - 1) / kBlock;
+  return {blocks, ((int64_t)R + U * kRowsAtOnce - 1) / (U * kRowsAtOnce) * blocks};
+}
+
+template <typename T, int N, int U>
+int run_forward_u(const void* x, int R, int I, void* y, void* q, float* scale, cudaStream_t s) {
+  const SwigluGrid g = swiglu_grid(R, I, U);
+  if (g.ctas > INT32_MAX) return MOE_ERR_TOO_LARGE;
+  auto kern = q ? swiglu_kernel<T, N, U, true> : swiglu_kernel<T, N, U, false>;
+  return cuda_status(launch_pdl(kern, dim3((unsigned)g.ctas), dim3(kThreads), 0, s, static_cast<const T*>(x), R, I,
+                                g.blocks, static_cast<T*>(y), static_cast<uint8_t*>(q), scale));
+}
+template <typename T, int N, int U>
+int run_backward_u(const void* dy, const void* q, const float* scale, int R, int I, void* dx, cudaStream_t s) {
+  const SwigluGrid g = swiglu_grid(R, I, U);
+  if (g.ctas > INT32_MAX) return MOE_ERR_TOO_LARGE;
+  return cuda_status(launch_pdl(swiglu_backward_kernel<T, N, U>, dim3((unsigned)g.ctas), dim3(kThreads), 0, s,
+                                static_cast<const T*>(dy), static_cast<const uint8_t*>(q), scale, R, I, g.blocks,
+                                static_cast<T*>(dx)));
+}
+
+template <typename T, int N>
+int run_forward(const void* x, int R, int I, void* y, void* q, float* scale, cudaStream_t s) {
+  return run_forward_u<T, N, 1>(x, R, I, y, q, scale, s);
+}
+template <typename T, int N>
+int run_backward(const void* dy, const void* q, const float* scale, int R, int I, void* dx, cudaStream_t s) {
+  return run_backward_u<T, N, 1>(dy, q, scale, R, I, dx, s);
+}
+
+// Columns a thread moves at a time: 16 bytes where the rows and halves allow it.
+template <typename T>
+int forward_typed(const void* x, int R, int I, void* y, void* q, float* scale, cudaStream_t s) {
+  constexpr int kMost = 16 / (int)sizeof(T);
+  int n = vector_elements(I, sizeof(T), kMost, {x, y});
+  n = vector_elements(I, 1, n, {q});
+  switch (n) {
+    case 8: if constexpr (kMost >= 8) return run_forward<T, 8>(x, R, I, y, q, scale, s);
+    case 4: return run_forward<T, 4>(x, R, I, y, q, scale, s);
+    case 2: return run_forward<T, 2>(x, R, I, y, q, scale, s);
+    default: return run_forward<T, 1>(x, R, I, y, q, scale, s);
+  }
+}
+template <typename T>
+int backward_typed(const void* dy, const void* q, const float* scale, int R, int I, void* dx, cudaStream_t s) {
+  constexpr int kMost = 16 / (int)sizeof(T);
+  int n = vector_elements(I, sizeof(T), kMost, {dy, dx});
+  n = vector_elements(I, 1, n, {q});
+  switch (n) {
+    case 8: if constexpr (kMost >= 8) return run_backward<T, 8>(dy, q, scale, R, I, dx, s);
+    case 4: return run_backward<T, 4>(dy, q, scale, R, I, dx, s);
+    case 2: return run_backward<T, 2>(dy, q, scale, R, I, dx, s);
+    default: return run_backward<T, 1>(dy, q, scale, R, I, dx, s);
+  }
+}
+
+int check_swiglu(int32_t R, int32_t I, int32_t dtype) {
+  if (R < 0 || I < 1 || !dtype_bytes(dtype)) return MOE_ERR_INVALID_ARGUMENT;
+  return I > INT32_MAX / 2 ? MOE_ERR_TOO_LARGE : MOE_OK;
+}
+
+}  // namespace
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" {
+
+MOE_API int moe_swiglu_forward(const void* x, int32_t num_rows, int32_t inter, int32_t dtype, void* y, void* codes,
+                               float* scales, void* stream) {
+  int st = check_swiglu(num_rows, inter, dtype);
+  if (st != MOE_OK) return st;
+  if (num_rows == 0) return MOE_OK;
+  if (!x || !y || !codes != !scales) return MOE_ERR_INVALID_ARGUMENT;
+  if (!aligned_to(x, dtype_bytes(dtype)) || !aligned_to(y, dtype_bytes(dtype)) || !aligned_to(scales, 4))
+    return MOE_ERR_MISALIGNED;
+  if ((st = require_device(nullptr)) != MOE_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == MOE_BF16) return forward_typed<__nv_bfloat16>(x, num_rows, inter, y, codes, scales, s);
+  if (dtype == MOE_F16) return forward_typed<__half>(x, num_rows, inter, y, codes, scales, s);
+  return forward_typed<float>(x, num_rows, inter, y, codes, scales, s);
+}
+
+MOE_API int moe_swiglu_backward(const void* grad_y, const void* codes, const float* scales, int32_t num_rows,
+                                int32_t inter, int32_t dtype, void* grad_x, void* stream) {
+  int st = check_swiglu(num_rows, inter, dtype);
+  if (st != MOE_OK) return st;
+  if (num_rows == 0) return MOE_OK;
+  if (!grad_y || !codes || !scales || !grad_x) return MOE_ERR_INVALID_ARGUMENT;
+  if (!aligned_to(grad_y, dtype_bytes(dtype)) || !aligned_to(grad_x, dtype_bytes(dtype)) || !aligned_to(scales, 4))
+    return MOE_ERR_MISALIGNED;
+  if ((st = require_device(nullptr)) != MOE_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == MOE_BF16) return backward_typed<__nv_bfloat16>(grad_y, codes, scales, num_rows, inter, grad_x, s);
+  if (dtype == MOE_F16) return backward_typed<__half>(grad_y, codes, scales, num_rows, inter, grad_x, s);
+  return backward_typed<float>(grad_y, codes, scales, num_rows, inter, grad_x, s);
+}
+
+}  // extern "C"

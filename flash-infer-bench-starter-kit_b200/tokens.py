@@ -54,9 +54,17 @@ def _check_order(order, device):
     return order.inv_row.shape
 
 
-def _combine(rows, weights, inv_row, out_dtype):
+def _dispatch(hidden, inv_row):
     T, K = inv_row.shape
-    out = torch.empty(T, rows.shape[1], dtype=out_dtype, device=rows.device)
+    rows = torch.empty(T * K, hidden.shape[1], dtype=hidden.dtype, device=hidden.device)
+    call("moe_tokens_dispatch", hidden.device, hidden, inv_row, T, K, hidden.shape[1], DTYPES[hidden.dtype], rows)
+    return rows
+
+
+def _combine(rows, weights, inv_row, out_dtype, out=None):
+    T, K = inv_row.shape
+    if out is None:
+        out = torch.empty(T, rows.shape[1], dtype=out_dtype, device=rows.device)
     call("moe_tokens_combine", rows.device, rows, inv_row, weights, T, K, rows.shape[1], DTYPES[rows.dtype],
          DTYPES[out_dtype], out)
     return out
@@ -65,11 +73,8 @@ def _combine(rows, weights, inv_row, out_dtype):
 class _Dispatch(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, inv_row):
-        T, K = inv_row.shape
-        rows = torch.empty(T * K, hidden.shape[1], dtype=hidden.dtype, device=hidden.device)
-        call("moe_tokens_dispatch", hidden.device, hidden, inv_row, T, K, hidden.shape[1], DTYPES[hidden.dtype], rows)
         ctx.save_for_backward(inv_row)
-        return rows
+        return _dispatch(hidden, inv_row)
 
     @staticmethod
     @once_differentiable
@@ -108,7 +113,9 @@ def dispatch(hidden_states: torch.Tensor, order: TokenOrder) -> torch.Tensor:
     T, _ = _check_order(order, hidden_states.device)
     if hidden_states.shape[0] != T:
         raise ValueError(f"hidden_states has {hidden_states.shape[0]} tokens, the order {T}")
-    return _Dispatch.apply(hidden_states, order.inv_row)
+    if hidden_states.requires_grad and torch.is_grad_enabled():
+        return _Dispatch.apply(hidden_states, order.inv_row)
+    return _dispatch(hidden_states, order.inv_row)
 
 
 def combine(rows: torch.Tensor, topk_weights: torch.Tensor, order: TokenOrder,
@@ -124,4 +131,6 @@ def combine(rows: torch.Tensor, topk_weights: torch.Tensor, order: TokenOrder,
     out_dtype = rows.dtype if out_dtype is None else out_dtype
     if out_dtype not in DTYPES or (out_dtype != rows.dtype and rows.dtype != torch.float32):
         raise TypeError(f"rows of {rows.dtype} cannot be combined to {out_dtype}")
-    return _Combine.apply(rows, topk_weights, order.inv_row, out_dtype)
+    if (rows.requires_grad or topk_weights.requires_grad) and torch.is_grad_enabled():
+        return _Combine.apply(rows, topk_weights, order.inv_row, out_dtype)
+    return _combine(rows, topk_weights, order.inv_row, out_dtype)

@@ -1,0 +1,163 @@
+"""Expert products with 4-bit weights, for decoding.
+
+Reading the experts' weights bounds a decode step of the layer, so 4-bit
+weights with group scales halve what its FP8 experts read:
+
+    w13 = W4Weights(*quantize_w4(w, group_size=128), group_size=128)   # once: [E, N, D] weights
+    y   = w4_matvec(rows, w13, order.offsets)     # rows sorted by expert (sort_tokens, dispatch)
+    out = moe_w4(hidden_states, topk_ids, topk_weights, w13, w2)       # the whole routed layer
+
+For inference only: there is no gradient.  The reference has no weights below
+8 bits.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from ._ops import DTYPES, call, check_tensor
+from .activation import swiglu
+from .tokens import _combine, dispatch, sort_tokens
+
+GROUP_SIZES = (32, 64, 128)
+_TILE_N, _TILE_K = 16, 64
+
+
+def quantize_w4(w: torch.Tensor, group_size: int, zero_points: bool = False, dtype: torch.dtype = torch.bfloat16):
+    """``(codes, scales, zeros)`` of weights ``w`` [..., N, D], each group of ``group_size`` columns to the
+    nearest of 16 values: codes uint8 [..., N, D / 2] (column 2j in the low half of byte j), scales
+    ``dtype`` [..., N, D / group_size] and, with ``zero_points``, zeros uint8 of the same shape (the code
+    that stands for 0; without, it is 8 and ``zeros`` is None)."""
+    if w.shape[-1] % group_size or group_size % 2:
+        raise ValueError(f"{w.shape[-1]} columns do not split into groups of {group_size}")
+    v = w.float().unflatten(-1, (-1, group_size))
+    if zero_points:
+        low, high = v.amin(-1).clamp_max(0), v.amax(-1).clamp_min(0)
+        scales = ((high - low) / 15).to(dtype)
+    else:
+        scales = (v.abs().amax(-1) / 7).to(dtype)
+    scales = torch.where(scales > 0, scales, torch.ones_like(scales))
+    s = scales.float()
+    zeros = torch.round(-low / s).clamp(0, 15) if zero_points else torch.full_like(s, 8)
+    q = (torch.round(v / s.unsqueeze(-1)) + zeros.unsqueeze(-1)).clamp(0, 15).to(torch.uint8).flatten(-2)
+    codes = q[..., 0::2] | (q[..., 1::2] << 4)
+    return codes, scales, zeros.to(torch.uint8) if zero_points else None
+
+
+def _pad(t, rows, cols):
+    return torch.nn.functional.pad(t, (0, cols - t.shape[1], 0, rows - t.shape[0]))
+
+
+class W4Weights:
+    """One 4-bit matrix per expert (``codes`` uint8 [E, N, D / 2], or [N, D / 2] for a single matrix), laid
+    out once for ``w4_matvec``.
+
+    Column 2j of a row is the low half of its byte j.  A weight is ``(code - zero) * scale`` with
+    ``scales`` [E, N, D / group_size] in fp16 or bf16, the type of the rows it will multiply, and
+    ``zeros`` uint8 of the same shape (0 to 15) or None for 8 everywhere."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, *,
+                 group_size: int):
+        if group_size not in GROUP_SIZES:
+            raise ValueError(f"group_size is {group_size}, expected one of {GROUP_SIZES}")
+        for name, t, dtypes in (("codes", codes, (torch.uint8,)), ("scales", scales, (torch.float16, torch.bfloat16)),
+                                ("zeros", zeros, (torch.uint8,))):
+            if t is None and name == "zeros":
+                continue
+            if not isinstance(t, torch.Tensor):
+                raise TypeError(f"{name} must be a torch.Tensor")
+            if t.dtype not in dtypes:
+                raise TypeError(f"{name} has dtype {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
+            if t.dim() not in (2, 3) or t.dim() != codes.dim() or t.device != codes.device:
+                raise ValueError(f"{name} must be [E, N, ...] or [N, ...], as and where the codes are")
+        if codes.dim() == 2:
+            codes, scales = codes.unsqueeze(0), scales.unsqueeze(0)
+            zeros = zeros.unsqueeze(0) if zeros is not None else None
+        E, N, D = codes.shape[0], codes.shape[1], codes.shape[2] * 2
+        if E < 1 or N < 1 or D < 1 or D % group_size:
+            raise ValueError(f"codes of shape {tuple(codes.shape)} do not split into groups of {group_size} columns")
+        for name, t in (("scales", scales), ("zeros", zeros)):
+            if t is not None and t.shape != (E, N, D // group_size):
+                raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {(E, N, D // group_size)}")
+        if zeros is not None and zeros.numel() and int(zeros.max()) > 15:
+            raise ValueError("zeros must be 0 to 15")
+        self.num_experts, self.n, self.d, self.group_size = E, N, D, group_size
+        self.dtype, self.device = scales.dtype, codes.device
+        n_tiles, k_tiles = -(-N // _TILE_N), -(-D // _TILE_K)
+        groups = k_tiles * _TILE_K // group_size
+        self.codes = torch.empty(E, n_tiles, k_tiles, 32, 16, dtype=torch.uint8, device=codes.device)
+        self.scales = torch.empty(E, n_tiles, groups, 8, 2, dtype=scales.dtype, device=codes.device)
+        self.zeros = torch.empty_like(self.scales, dtype=torch.uint8) if zeros is not None else None
+        for e in range(E):
+            self._lay_out(e, codes[e], scales[e], zeros[e] if zeros is not None else None, n_tiles, k_tiles, groups)
+
+    def _lay_out(self, e, codes, scales, zeros, n_tiles, k_tiles, groups):
+        rows = n_tiles * _TILE_N
+        c = _pad(codes, rows, k_tiles * _TILE_K // 2)
+        q = torch.stack([c & 15, c >> 4], dim=2)
+        # (tile, row half, g; tile, h, t, word, pair, place) -> lane (g, t), word (h, word), nibble (place, pair, row half)
+        q = q.view(n_tiles, 2, 8, k_tiles, 2, 4, 2, 2, 2).permute(0, 3, 2, 5, 4, 6, 8, 7, 1)
+        self.codes[e].view(n_tiles, k_tiles, 8, 4, 2, 2, 2, 2).copy_(q[..., 0] | (q[..., 1] << 4))
+        for out, t in ((self.scales, scales), (self.zeros, zeros)):
+            if t is not None:
+                out[e].copy_(_pad(t, rows, groups).view(n_tiles, 2, 8, groups).permute(0, 3, 2, 1))
+
+
+def w4_matvec(x: torch.Tensor, weights: W4Weights, offsets: torch.Tensor | None = None,
+              out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``y[r] = W[e] x[r]`` for the rows ``offsets[e] <= r < offsets[e + 1]`` of each expert e ([R, N]), in
+    fp32, rounded once to ``out_dtype`` (``x``'s type or fp32).
+
+    ``x`` [R, D] has the weights' type; ``offsets`` int32 [E + 1] as ``sort_tokens`` gives them, None for a
+    single matrix.  Rows outside ``[offsets[0], offsets[E])`` are zero in a new result and left as they
+    were in a given ``out``.  The weights of each expert with rows are read once for up to 32 rows, so
+    this is the product for decode batches; prefill batches want a GEMM."""
+    if not isinstance(weights, W4Weights):
+        raise TypeError("weights must be W4Weights")
+    check_tensor("x", x, (weights.dtype,), (-1, weights.d), None)
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError("w4_matvec has no gradient: detach x or call it under torch.no_grad()")
+    dev = x.device
+    if weights.device != dev:
+        raise ValueError(f"weights are on {weights.device}, expected {dev}")
+    if offsets is not None:
+        check_tensor("offsets", offsets, (torch.int32,), (weights.num_experts + 1,), dev)
+    elif weights.num_experts != 1:
+        raise ValueError(f"{weights.num_experts} experts need offsets")
+    R, fresh = x.shape[0], out is None
+    if fresh:
+        out_dtype = x.dtype if out_dtype is None else out_dtype
+        if out_dtype not in (x.dtype, torch.float32):
+            raise TypeError(f"out_dtype is {out_dtype}, expected {x.dtype} or torch.float32")
+        out = torch.empty(R, weights.n, dtype=out_dtype, device=dev)
+    else:
+        check_tensor("out", out, (x.dtype, torch.float32) if out_dtype is None else (out_dtype,), (R, weights.n), dev)
+    if x.data_ptr() % 16:
+        x = x.clone()
+    call("moe_w4_matvec", dev, x, weights.codes, weights.scales, weights.zeros, offsets, R, weights.num_experts,
+         weights.n, weights.d, weights.group_size, DTYPES[x.dtype], DTYPES[out.dtype], int(fresh), out)
+    return out
+
+
+def moe_w4(hidden_states: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tensor, w13: W4Weights,
+           w2: W4Weights, local_expert_offset: int = 0, output: torch.Tensor | None = None) -> torch.Tensor:
+    """The routed layer with 4-bit experts: ``sum_k topk_weights[t, k] * W2[e] swiglu(W13[e] hidden[t])``
+    over the experts ``e = topk_ids[t, k]`` on this shard ([T, H], the type of ``hidden_states``; written
+    to ``output`` if given).  ``w13`` [E, 2 * I, H] holds up's rows, then gate's."""
+    for name, w in (("w13", w13), ("w2", w2)):
+        if not isinstance(w, W4Weights):
+            raise TypeError(f"{name} must be W4Weights")
+    if w13.num_experts != w2.num_experts or w13.n != 2 * w2.d:
+        raise ValueError(f"w13 has {w13.num_experts} experts of {w13.n} rows, w2 {w2.num_experts} of {w2.d} columns")
+    if hidden_states.requires_grad and torch.is_grad_enabled():
+        raise ValueError("moe_w4 has no gradient: detach hidden_states or call it under torch.no_grad()")
+    order = sort_tokens(topk_ids, w13.num_experts, local_expert_offset)
+    T, K = topk_ids.shape
+    check_tensor("topk_weights", topk_weights, (torch.float32,), (T, K), topk_ids.device)
+    check_tensor("hidden_states", hidden_states, (w13.dtype,), (T, w13.d), topk_ids.device)
+    if output is not None:
+        check_tensor("output", output, (hidden_states.dtype,), (T, w2.n), topk_ids.device)
+    rows = w4_matvec(dispatch(hidden_states, order), w13, order.offsets)
+    # fp32 from the second product to the sum over k: one rounding, as in the fused layer
+    down = w4_matvec(swiglu(rows), w2, order.offsets, out_dtype=torch.float32)
+    return _combine(down, topk_weights.detach(), order.inv_row, hidden_states.dtype, output)

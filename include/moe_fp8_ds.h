@@ -299,6 +299,38 @@ MOE_API int moe_tokens_combine_backward(const void* grad_out, const void* rows, 
                                         int32_t rows_dtype, int32_t out_dtype, void* grad_rows,
                                         float* grad_weights, void* stream);
 
+/* SwiGLU of rows x = [up | gate] (each [R, inter]): y = up * gate * sigmoid(gate).
+ * With codes and scales (both or neither), x is kept for the backward pass in
+ * 8 bits: each 1x128 block of up and of gate (the last may be shorter) as e4m3
+ * codes [R, 2 * inter] with scale amax / 448 (1 for a zero block), scales fp32
+ * [2 * ceil(inter / 128), R], up's blocks first.  A block with an infinity or a
+ * NaN is kept as NaN.                                                        */
+MOE_API int moe_swiglu_forward(const void* x, int32_t num_rows, int32_t inter, int32_t dtype, void* y, void* codes,
+                               float* scales, void* stream);
+
+/* grad_x [R, 2 * inter] from grad_y [R, inter] and what the forward call kept. */
+MOE_API int moe_swiglu_backward(const void* grad_y, const void* codes, const float* scales, int32_t num_rows,
+                                int32_t inter, int32_t dtype, void* grad_x, void* stream);
+
+/* Products of few rows with 4-bit weights: y[r, n] = sum over groups of
+ * scale[e, n, group] * sum over the group's k of (code[e, n, k] - zero[e, n, group]) * x[r, k]
+ * for the rows offsets[e] <= r < offsets[e + 1] of expert e; offsets NULL means
+ * one matrix for all rows.  x [R, d] and the scales are fp16 or bf16 (dtype), y
+ * [R, n] has that type or fp32 (out_dtype).  Sums are fp32, rounded once.
+ * group_size is 32, 64 or 128 and divides d.  Layout, with N = n rounded up to 16 and
+ * D = d rounded up to 64 (all padding zero): codes [E][N / 16][D / 64][32 lanes][16
+ * bytes]; lane 4 * g + t holds, in 32-bit word j, columns c = 32 * (j / 2) + 8 * t +
+ * 4 * (j % 2) + {0, 1, 2, 3} of rows g and g + 8 as nibbles 0, 4 = (g; c, c + 1),
+ * 1, 5 = (g + 8; c, c + 1), 2, 6 = (g; c + 2, c + 3), 3, 7 = (g + 8; c + 2, c + 3);
+ * scales [E][N / 16][D / group_size][8][2] (rows g and g + 8 of a tile together);
+ * zeros uint8, laid out as the scales, or NULL: 8.  Rows of x outside
+ * [offsets[0], offsets[E]) get zeros when zero_other_rows is set, else their y is left as
+ * it was.  num_experts <= 1024.                                               */
+MOE_API int moe_w4_matvec(const void* x, const void* codes, const void* scales, const void* zeros,
+                          const int32_t* offsets, int32_t num_rows, int32_t num_experts, int32_t n, int32_t d,
+                          int32_t group_size, int32_t dtype, int32_t out_dtype, int32_t zero_other_rows, void* y,
+                          void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -51,3 +51,117 @@ def test_token_entries_check_their_arguments(pkg):
     assert back(p, p, p, None, 4, 8, 16, L.MOE_F32, L.MOE_F32, p, p, None) == bad
     assert back(p, p, p, p, 4, 8, 16, L.MOE_F32, L.MOE_F32, None, None, None) == L.MOE_OK
     assert back(p, p, p, p, 4, 8, 16, L.MOE_F32, L.MOE_F32, p + 2, p, None) == odd
+
+
+def test_swiglu_and_w4_entries_check_their_arguments(pkg):
+    L = sys.modules["fib_b200._lib"]
+    lib, bad, big, odd = L.load(), L.MOE_ERR_INVALID_ARGUMENT, L.MOE_ERR_TOO_LARGE, L.MOE_ERR_MISALIGNED
+    p = 64
+    fwd, bwd = lib.moe_swiglu_forward, lib.moe_swiglu_backward
+    assert fwd(p, -1, 8, L.MOE_BF16, p, None, None, None) == bad
+    assert fwd(p, 4, 0, L.MOE_BF16, p, None, None, None) == bad
+    assert fwd(p, 4, 8, 9, p, None, None, None) == bad
+    assert fwd(p, 4, 8, L.MOE_BF16, p, p, None, None) == bad
+    assert fwd(p, 4, 8, L.MOE_BF16, p, None, p, None) == bad
+    assert fwd(p + 1, 4, 8, L.MOE_BF16, p, None, None, None) == odd
+    assert fwd(p, 4, 1 << 30, L.MOE_BF16, p, None, None, None) == big
+    assert fwd(None, 0, 8, L.MOE_BF16, None, None, None, None) == L.MOE_OK
+    assert bwd(p, None, p, 4, 8, L.MOE_BF16, p, None) == bad
+    assert bwd(p, p, p + 2, 4, 8, L.MOE_BF16, p, None) == odd
+    assert bwd(None, None, None, 0, 8, L.MOE_BF16, None, None) == L.MOE_OK
+    mv = lib.moe_w4_matvec
+
+    def call(x=p, codes=p, scales=p, zeros=None, offsets=p, R=4, E=2, n=16, d=128, group=64, dt=L.MOE_BF16,
+             out=L.MOE_BF16, y=p):
+        return mv(x, codes, scales, zeros, offsets, R, E, n, d, group, dt, out, 0, y, None)
+    assert call(R=-1) == call(E=0) == call(n=0) == call(d=0) == bad
+    assert call(group=16) == call(group=256) == call(d=96) == bad
+    assert call(offsets=None) == bad
+    assert call(dt=L.MOE_F32) == call(out=L.MOE_F16) == bad
+    assert call(codes=None) == call(x=None) == call(scales=None) == call(y=None) == bad
+    assert call(E=1025) == big
+    assert call(x=p + 2) == call(codes=p + 8) == call(scales=p + 2) == call(zeros=p + 1) == call(y=p + 1) == odd
+    assert call(R=0, x=None, y=None) == L.MOE_OK
+
+
+def test_swiglu_and_w4_refuse_cpu_tensors_and_shapes(pkg):
+    with pytest.raises(ValueError, match="CUDA"):
+        pkg.swiglu(torch.zeros(2, 8))
+    codes, scales, _ = pkg.quantize_w4(torch.randn(3, 20, 64), 32)
+    w = pkg.W4Weights(codes, scales, group_size=32)
+    assert (w.num_experts, w.n, w.d, w.dtype) == (3, 20, 64, torch.bfloat16)
+    with pytest.raises(ValueError, match="CUDA"):
+        pkg.w4_matvec(torch.zeros(2, 64, dtype=torch.bfloat16), w)
+    with pytest.raises(TypeError):
+        pkg.w4_matvec(torch.zeros(2, 64, dtype=torch.float16), w)
+    with pytest.raises(ValueError):
+        pkg.w4_matvec(torch.zeros(2, 32, dtype=torch.bfloat16), w)
+    with pytest.raises(TypeError):
+        pkg.w4_matvec(torch.zeros(2, 64), (codes, scales))
+    with pytest.raises(ValueError):
+        pkg.quantize_w4(torch.randn(4, 100), 32)
+    W = pkg.W4Weights
+    with pytest.raises(ValueError):
+        W(codes, scales, group_size=16)
+    with pytest.raises(ValueError):
+        W(codes, scales, group_size=64)
+    with pytest.raises(ValueError):
+        W(codes[:, :, :8], scales, group_size=32)
+    with pytest.raises(ValueError):
+        W(codes, scales[0], group_size=32)
+    with pytest.raises(ValueError):
+        W(codes, scales, torch.full(scales.shape, 16, dtype=torch.uint8), group_size=32)
+    with pytest.raises(TypeError):
+        W(codes, scales.float(), group_size=32)
+    with pytest.raises(TypeError):
+        W(codes.to(torch.int8), scales, group_size=32)
+
+
+@pytest.mark.parametrize("zero_points", [False, True])
+@pytest.mark.parametrize("N,D,group", [(16, 64, 64), (20, 96, 32), (33, 256, 128), (1, 32, 32)])
+def test_w4_layout_is_the_documented_one(N, D, group, zero_points, pkg):
+    """Every code, scale and zero point is where the header says, padding is zero."""
+    g = torch.Generator().manual_seed(N + D)
+    E = 2
+    codes = torch.randint(0, 256, (E, N, D // 2), generator=g, dtype=torch.uint8)
+    scales = torch.randn(E, N, D // group, generator=g).to(torch.float16)
+    zeros = torch.randint(0, 16, scales.shape, generator=g, dtype=torch.uint8) if zero_points else None
+    w = pkg.W4Weights(codes, scales, zeros, group_size=group)
+    n16, d64 = -(-N // 16) * 16, -(-D // 64) * 64
+    got = torch.zeros(E, n16, d64, dtype=torch.uint8)
+    words = w.codes.reshape(E, n16 // 16, d64 // 64, 32, 16).numpy().view("<u4")
+    for tile in range(n16 // 16):
+        for kt in range(d64 // 64):
+            for lane in range(32):
+                row, t = lane // 4, lane % 4
+                for j in range(4):
+                    c = kt * 64 + 32 * (j // 2) + 8 * t + 4 * (j % 2)
+                    for nib, (r, k) in {0: (0, 0), 4: (0, 1), 1: (8, 0), 5: (8, 1), 2: (0, 2), 6: (0, 3), 3: (8, 2),
+                                        7: (8, 3)}.items():
+                        for e in range(E):
+                            got[e, tile * 16 + row + r, c + k] = (int(words[e, tile, kt, lane, j]) >> (4 * nib)) & 15
+    want = torch.zeros_like(got)
+    want[:, :N, 0:D:2], want[:, :N, 1:D:2] = codes & 15, codes >> 4
+    assert torch.equal(got, want)
+    for packed, plain in ((w.scales, scales), (w.zeros, zeros)):
+        if plain is None:
+            assert packed is None
+            continue
+        full = torch.zeros(E, n16, d64 // group, dtype=plain.dtype)
+        full[:, :N, :D // group] = plain
+        assert torch.equal(packed.permute(0, 1, 4, 3, 2).reshape(E, n16, -1), full)
+
+
+@pytest.mark.parametrize("zero_points", [False, True])
+def test_quantize_w4_takes_the_nearest_value(zero_points, pkg):
+    g = torch.Generator().manual_seed(5)
+    w = torch.randn(2, 10, 96, generator=g)
+    w[0, 0] = 0
+    codes, scales, zeros = pkg.quantize_w4(w, 32, zero_points)
+    q = torch.stack([codes & 15, codes >> 4], -1).flatten(-2).unflatten(-1, (3, 32)).float()
+    z = zeros.unsqueeze(-1).float() if zero_points else 8.0
+    back = ((q - z) * scales.unsqueeze(-1).float()).flatten(-2)
+    step = scales.float().repeat_interleave(32, -1)
+    # half a step, and at an end of the range what the rounding of the scale (bf16, 2^-8) over 15 codes and
+    # of the zero point (half a step) clips
+    assert bool(((w - back).abs() <= step * (0.5 + 15 * 2.0 ** -8 + (0.5 if zero_points else 0.0))).all())
