@@ -3,218 +3,245 @@
 // group of G columns)
 //   y[r, n] = sum over groups g of scale[e,n,g] * sum_{k in g} (q[e,n,k] - zero[e,n,g]) * x[r,k].
 //
-// The weights of the experts that have rows are read once, and reading them
-// bounds the product up to about 16 rows an expert (4 bits a weight against
-// 2 * rows operations).  Rows are few, so weights are on the M side of
-// mma.sync m16n8k16 (tcgen05 would need the decoded weights in shared memory or
-// TMEM, eight times the bytes that are read, to multiply tiles of mostly
-// missing rows): codes go from memory to registers, become the exact 16-bit
-// values q - zero there, and multiply up to 8 rows of x at a time.  A group's
-// sum is made in fp32 and scaled in fp32, so nothing is rounded before the output.
+// The codes of the experts that have rows are read once, and reading them should
+// bound the product, so the work on each code has to be small.  It is with fp16
+// operands (mma.sync m16n8k16, fp32 sums, weights on the M side): the number 0..15 in
+// the low bits of an fp16 is exactly q * 2^-24 (below 2^-14 fp16 is evenly
+// spaced), four bits higher it is 16 * q * 2^-24, so a 32-bit word of eight codes
+// becomes four operand registers by four masks, one shift and four subtractions of
+// the zero point, all exact.  The factors 2^24 and 1/16 go into the scales and the
+// last step; a group's sum is scaled in fp32, and only the output is rounded.
+// (e4m3 operands, where a byte 0..15 is q * 2^-9, need half the masks, but mma.sync
+// with e4m3 is converted to fp16 here: measured four times the instructions.
+// tcgen05 would want the decoded weights in shared memory or TMEM and 128-row tiles; a
+// decode batch has too few rows of x for that to pay.)
+//
+// fp16 rows of x are the other operand as they are.  bf16 rows are first brought
+// to fp16 by a power of two for each row that puts its largest magnitude into
+// [2^14, 2^15): exact for values down to 2^-28 of the largest, below that off by at
+// most 2^-39 of it.  (Next to an infinity or a NaN the finite values vanish, as they
+// do in the sum.)
 //
 // Layout (made once, by the caller): 16 x 64 tiles of codes in the order in
 // which a warp's lanes take them, 16 bytes a lane.  With lane = 4 * g + t, 32-bit
-// word j holds columns c = 32 * (j / 2) + 8 * t + 4 * (j % 2) + {0, 1, 2, 3} of
-// rows g and g + 8: nibbles 0, 4 = (g; c, c + 1), 1, 5 = (g + 8; c, c + 1), 2, 6 =
-// (g; c + 2, c + 3), 3, 7 = (g + 8; c + 2, c + 3), so that (word >> 4i) & 0x000f000f
-// is the i-th A register of step j, and a lane's B registers are 16 consecutive
-// bytes of x.  Scales are [E][N / 16][groups][8][2] (rows g, g + 8 together), zero
-// points likewise.
+// word j holds columns c = 32 * (j / 2) + 8 * t + 4 * (j % 2) + {0, 2, 1, 3} in its
+// bytes 0 to 3, row g in the low half of a byte and row g + 8 in the high half: a
+// lane's share of x is then 16 consecutive bytes for each 32 columns.  Scales are
+// [E][N / 16][groups][8][2] (rows g, g + 8 together), zero points likewise.
 #include "rows.cuh"
 
 namespace moe {
 namespace {
 
-constexpr int kW4Threads = 256;
-constexpr int kW4Warps = kW4Threads / 32;
-constexpr int kMaxRows = 32;              // rows of x in one unit of work
-constexpr int kMaxExperts = 1024;
+constexpr int kWarps = 8;                 // of a CTA; they split the columns
+constexpr int kThreads = kWarps * 32;
+constexpr int kCtasPerSm = 2;
+constexpr int kM = 4;                     // 16-row tiles of weights in a task
+constexpr int kMaxRows = 16;              // rows of x in a task
+constexpr int kStages = 4;                // of a warp's ring of tiles
 constexpr int kTileK = 64;                // columns of a tile
-constexpr int kUnitTiles = 4;             // 16-row tiles of a unit
-constexpr int kSumFloats = 1152;          // a warp's sums: 16 rows x 68 or 32 rows x 36, padded
+constexpr int kMaxExperts = 1024;
+constexpr int kSumM = 2;                  // rows of tiles whose sums are joined at a time
+constexpr int kSumStride = kSumM * 16 + 4;   // of the sums in shared memory: a warp's stores hit 32 banks
 
 struct W4Params {
-  const void* x;
+  const __half* x;         // [R, D]
+  const int32_t* row_exp;  // [R]: the exponent taken out of a bf16 row, or null: 0
   const uint4* codes;      // [E][n_tiles][k_tiles][32]
   const uint32_t* scales;  // [E][n_tiles][groups][8] pairs of 16-bit scales
-  const uint16_t* zeros;   // [E][n_tiles][groups][8] pairs of 8-bit zero points, or null
+  const uint32_t* zeros;   // [E][n_tiles][groups][4] pairs of pairs of 8-bit zero points, or null
   const int32_t* offsets;  // [E + 1], or null: one matrix for all rows
   void* y;
   int R, N, D, E, n_tiles, k_tiles, groups, group_shift;
   int out_f32, zero_rest;
 };
 
-template <typename T> struct Half2;
-template <> struct Half2<__nv_bfloat16> {
-  static constexpr uint32_t kBase = 0x43004300u;   // 128, 128: the last mantissa bits count ones
-  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-    uint32_t d;
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    return d;
-  }
-  static __device__ __forceinline__ float2 scales(uint32_t v) {
-    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
-  }
-  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-};
-template <> struct Half2<__half> {
-  static constexpr uint32_t kBase = 0x64006400u;   // 1024, 1024
-  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-    uint32_t d;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    return d;
-  }
-  static __device__ __forceinline__ float2 scales(uint32_t v) {
-    return __half22float2(*reinterpret_cast<__half2*>(&v));
-  }
-  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-};
+// --------------------------------------------------------------------------
+// bf16 rows to fp16: a CTA takes a row, finds its largest magnitude and scales by
+// 2^-exp.  Reads and writes R * D * 2 bytes, a few microseconds of latency.
+// --------------------------------------------------------------------------
+constexpr int kConvertThreads = 256;
 
-__device__ __forceinline__ uint4 load_codes(const uint4* p) {   // read once
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
+__global__ void __launch_bounds__(kConvertThreads)
+w4_convert_kernel(const __nv_bfloat16* __restrict__ x, int D, __half* __restrict__ out, int32_t* __restrict__ row_exp) {
+  __shared__ float s_max[kConvertThreads / 32];
+  griddep_wait();
+  griddep_launch_dependents();
+  const size_t base = (size_t)blockIdx.x * D;
+  float amax = 0.f;
+  for (int i = threadIdx.x * 8; i < D; i += kConvertThreads * 8) {   // D is a multiple of 32
+    const Pack<__nv_bfloat16, 8> v = load_cached<__nv_bfloat16, 8>(x + base + i);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float a = fabsf(to_float(v.v[j]));
+      amax = a < INFINITY ? fmaxf(amax, a) : INFINITY;
+    }
+  }
+#pragma unroll
+  for (int off = 16; off; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = amax;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kConvertThreads / 32; ++i) amax = fmaxf(amax, s_max[i]);
+  // amax * 2^-exp in [2^14, 2^15), as far as 2^-exp is a normal number
+  int exp = (int)((__float_as_uint(amax) >> 23) & 0xff) - 127 - 14;
+  exp = exp < -120 ? -120 : exp;
+  const float down = __uint_as_float((uint32_t)(127 - exp) << 23);
+  for (int i = threadIdx.x * 8; i < D; i += kConvertThreads * 8) {
+    const Pack<__nv_bfloat16, 8> v = load_cached<__nv_bfloat16, 8>(x + base + i);
+    Pack<__half, 8> h;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) h.v[j] = __float2half_rn(to_float(v.v[j]) * down);
+    store_wide<__half, 8>(out + base + i, h);
+  }
+  if (threadIdx.x == 0) row_exp[blockIdx.x] = exp;
 }
 
-// One warp's part of a unit: MT tiles of 16 weight rows times NT * 8 rows of x
-// over the tiles [k0, k1) of columns; sums[mt][nt] are the mma's C registers.
-template <typename T, int NT, int MT, bool SMALL, bool ZEROS>
-__device__ __forceinline__ void warp_product(const W4Params& p, int e, int m0, int r0, int cnt, int k0, int k1,
-                                             float (&sums)[MT][NT][4]) {
-  using H = Half2<T>;
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const size_t tile0 = (size_t)e * p.n_tiles + m0;
-  const uint4* codes = p.codes + tile0 * p.k_tiles * 32 + lane;
-  const uint32_t* scales = p.scales + tile0 * p.groups * 8 + g;
-  const uint16_t* zeros = ZEROS ? p.zeros + tile0 * p.groups * 8 + g : nullptr;
-  const int m_here = p.n_tiles - m0 < MT ? p.n_tiles - m0 : MT;
-  const uint4* x[NT];
+// --------------------------------------------------------------------------
+// The product.
+// --------------------------------------------------------------------------
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                        uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {   // subnormal numbers included
+  uint32_t d;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+// Asynchronous copies to shared memory.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <typename T> __device__ __forceinline__ float2 pair_of(uint32_t v);
+template <> __device__ __forceinline__ float2 pair_of<__nv_bfloat16>(uint32_t v) {
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+template <> __device__ __forceinline__ float2 pair_of<__half>(uint32_t v) {
+  return __half22float2(*reinterpret_cast<__half2*>(&v));
+}
+
+// One step of a warp's ring: a tile of each of kM rows of tiles, their scales and
+// zero points.
+template <bool SMALL, bool ZEROS>
+struct Stage {
+  static constexpr int kParts = SMALL ? 2 : 1;   // groups in a tile
+  uint4 codes[kM][32];
+  uint32_t scales[kParts][kM][8];
+  uint32_t zeros[ZEROS ? kParts : 1][kM][4];
+};
+
+// A task: tiles [m0, m0 + m) of rows of expert e's matrix, times rows [r0, r0 + cnt) of x.
+struct Task {
+  int e, m0, m, r0, cnt;
+};
+
+// Start the copies of tile k of a task.
+template <bool SMALL, bool ZEROS>
+__device__ __forceinline__ void fill(const W4Params& p, const Task& w, int k, Stage<SMALL, ZEROS>* st) {
+  const int lane = threadIdx.x & 31;
+  const size_t tile0 = (size_t)w.e * p.n_tiles + w.m0;
+  const uint4* codes = p.codes + (tile0 * p.k_tiles + k) * 32 + lane;
+#pragma unroll
+  for (int m = 0; m < kM; ++m)
+    if (m < w.m) copy16(smem_u32(&st->codes[m][lane]), codes + (size_t)m * p.k_tiles * 32);
+#pragma unroll
+  for (int part = 0; part < Stage<SMALL, ZEROS>::kParts; ++part) {
+    const int group = (k * kTileK + part * 32) >> p.group_shift;
+    const int m = lane >> 3, g = lane & 7;
+    if (m < w.m) copy4(smem_u32(&st->scales[part][m][g]), p.scales + ((tile0 + m) * p.groups + group) * 8 + g);
+    if (ZEROS) {
+      const int mz = (lane >> 2) & 3, gz = lane & 3;
+      if (lane < 16 && mz < w.m)
+        copy4(smem_u32(&st->zeros[part][mz][gz]), p.zeros + ((tile0 + mz) * p.groups + group) * 4 + gz);
+    }
+  }
+}
+
+// A lane's share of a tile's columns of x: rows nt * 8 + g of the task, columns 8 t .. + 7 of each 32.
+template <int NT>
+__device__ __forceinline__ void load_x(const W4Params& p, const __half* const (&rows)[NT], int k, uint4 (&x)[NT][2]) {
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
-    x[nt] = nt * 8 + g < cnt
-                ? reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + (size_t)(r0 + nt * 8 + g) * p.D) + t
-                : nullptr;
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sums[mt][nt][i] = 0.f;
-  uint4 next[MT];
-  auto fetch = [&](int k) {
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-      if (mt < m_here) next[mt] = load_codes(codes + ((size_t)mt * p.k_tiles + k) * 32);
-  };
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) next[mt] = make_uint4(0, 0, 0, 0);
-  if (k0 < k1) fetch(k0);
-#pragma unroll 1
-  for (int k = k0; k < k1; ++k) {
-    uint32_t word[MT][4];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      word[mt][0] = next[mt].x; word[mt][1] = next[mt].y; word[mt][2] = next[mt].z; word[mt][3] = next[mt].w;
+    for (int h = 0; h < 2; ++h) {
+      const int col = k * kTileK + h * 32;
+      x[nt][h] = rows[nt] && col < p.D ? __ldg(reinterpret_cast<const uint4*>(rows[nt] + col)) : make_uint4(0, 0, 0, 0);
     }
-    if (k + 1 < k1) fetch(k + 1);
-    uint4 b[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        b[nt][h] = x[nt] && k * kTileK + 32 * h < p.D ? __ldg(x[nt] + k * 8 + h * 4) : make_uint4(0, 0, 0, 0);
-    constexpr int kParts = SMALL ? 2 : 1;       // groups of 32 columns: two in a tile
-#pragma unroll
-    for (int part = 0; part < kParts; ++part) {
-      const int group = (k * kTileK + part * 32) >> p.group_shift;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        if (mt >= m_here) continue;
-        const size_t at = ((size_t)mt * p.groups + group) * 8;
-        const float2 s = H::scales(__ldg(scales + at));
-        uint32_t z0 = H::kBase | 0x00080008u, z1 = z0;
-        if (ZEROS) {
-          const uint32_t z = __ldg(zeros + at);
-          z0 = H::kBase | (z & 0xff) * 0x00010001u;
-          z1 = H::kBase | (z >> 8) * 0x00010001u;
-        }
-        float c[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) c[nt][i] = 0.f;
-#pragma unroll
-        for (int j = part * 2; j < (SMALL ? part * 2 + 2 : 4); ++j) {
-          uint32_t a[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            a[i] = H::sub(((word[mt][j] >> (4 * i)) & 0x000f000fu) | H::kBase, (i & 1) ? z1 : z0);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const uint4 v = b[nt][j >> 1];
-            H::mma(c[nt], a, (j & 1) ? v.z : v.x, (j & 1) ? v.w : v.y);
-          }
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sums[mt][nt][i] = fmaf(i < 2 ? s.x : s.y, c[nt][i], sums[mt][nt][i]);
-      }
-    }
-  }
 }
 
-// A unit: kUnitN weight rows of expert e from row n0, rows [r0, r0 + cnt) of x.
-// The warps split the columns; their sums meet in shared memory and are added in
-// warp order.
-template <typename T, int NT, int MT, bool SMALL, bool ZEROS>
-__device__ __forceinline__ void run_unit(const W4Params& p, int e, int m0, int m1, int r0, int cnt, float* s_out) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int k0 = (int)((int64_t)p.k_tiles * warp / kW4Warps), k1 = (int)((int64_t)p.k_tiles * (warp + 1) / kW4Warps);
-  constexpr int kStride = MT * 16 + 4;   // of the sums in shared memory: a warp's stores hit 32 banks
-  static_assert(NT * 8 * kStride <= kSumFloats, "sums of a unit");
-  for (int m = m0; m < m1; m += MT) {
-    float sums[MT][NT][4];
-    warp_product<T, NT, MT, SMALL, ZEROS>(p, e, m, r0, cnt, k0, k1, sums);
-    float* mine = s_out + (size_t)warp * kSumFloats;
+template <typename T, int NT, bool SMALL, bool ZEROS>
+__device__ __forceinline__ void multiply(const Stage<SMALL, ZEROS>* st, int m_here, const uint4 (&x)[NT][2],
+                                         float (&sums)[kM][NT][4]) {
+  const int lane = threadIdx.x & 31, g = lane >> 2;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+  for (int m = 0; m < kM; ++m) {
+    if (m >= m_here) break;
+    const uint4 c = st->codes[m][lane];
+    const uint32_t word[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+    for (int part = 0; part < Stage<SMALL, ZEROS>::kParts; ++part) {
+      uint32_t z0 = 0x00080008u, z1 = 0x00800080u;   // zero points, row g + 8's times 16 as its codes are
+      if (ZEROS) {
+        const uint32_t z = st->zeros[part][m][g >> 1] >> (16 * (g & 1));
+        z0 = (z & 0xff) * 0x00010001u;
+        z1 = (z >> 8 & 0xff) * 0x00100010u;
+      }
+      float a[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          mine[(nt * 8 + 2 * t + (i & 1)) * kStride + mt * 16 + g + 8 * (i >> 1)] = sums[mt][nt][i];
-    __syncthreads();
-    for (int o = threadIdx.x; o < cnt * MT * 16; o += kW4Threads) {
-      const int row = o / (MT * 16), n = o % (MT * 16), col = m * 16 + n;
-      float v = 0.f;
+        for (int i = 0; i < 4; ++i) a[nt][i] = 0.f;
 #pragma unroll
-      for (int w = 0; w < kW4Warps; ++w) v += s_out[w * kSumFloats + row * kStride + n];
-      if (col >= p.N) continue;
-      const size_t at = (size_t)(r0 + row) * p.N + col;
-      if (p.out_f32) static_cast<float*>(p.y)[at] = v;
-      else static_cast<T*>(p.y)[at] = from_float<T>(v);
+      for (int j = 2 * part; j < (SMALL ? 2 * part + 2 : 4); ++j) {
+        const uint32_t w = word[j], w8 = w >> 8;
+        const uint32_t a0 = sub_f16x2(w & 0x000f000fu, z0), a1 = sub_f16x2(w & 0x00f000f0u, z1);
+        const uint32_t a2 = sub_f16x2(w8 & 0x000f000fu, z0), a3 = sub_f16x2(w8 & 0x00f000f0u, z1);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint4 v = x[nt][j >> 1];
+          mma_f16(a[nt], a0, a1, a2, a3, (j & 1) ? v.z : v.x, (j & 1) ? v.w : v.y);
+        }
+      }
+      float2 s = pair_of<T>(st->scales[part][m][g]);
+      s.y *= 0.0625f;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {      // rows g and g + 8; two rows of x in each fma
+          const float2 sum = __ffma2_rn(make_float2(a[nt][2 * h], a[nt][2 * h + 1]),
+                                        h ? make_float2(s.y, s.y) : make_float2(s.x, s.x),
+                                        make_float2(sums[m][nt][2 * h], sums[m][nt][2 * h + 1]));
+          sums[m][nt][2 * h] = sum.x;
+          sums[m][nt][2 * h + 1] = sum.y;
+        }
     }
-    __syncthreads();
   }
 }
 
+template <bool SMALL, bool ZEROS>
+constexpr size_t kRingBytes = sizeof(Stage<SMALL, ZEROS>) * kStages * kWarps;
+constexpr size_t kSumBytes = sizeof(float) * kWarps * kMaxRows * kSumStride;
+
 template <typename T, bool SMALL, bool ZEROS>
-__global__ void __launch_bounds__(kW4Threads, 2) w4_kernel(const W4Params p) {
-  __shared__ float s_out[kW4Warps * kSumFloats];
-  __shared__ int s_units[kMaxExperts + 1];
-  griddep_wait();
-  griddep_launch_dependents();
-  const int blocks = (p.n_tiles + kUnitTiles - 1) / kUnitTiles;
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) w4_kernel(const W4Params p) {
+  using St = Stage<SMALL, ZEROS>;
+  extern __shared__ __align__(16) uint8_t s_mem[];
+  __shared__ int s_chunks[kMaxExperts + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  St* ring = reinterpret_cast<St*>(s_mem) + warp * kStages;
+  float* s_sums = reinterpret_cast<float*>(s_mem + kRingBytes<SMALL, ZEROS>);
+
   auto rows_of = [&](int e, int* first) {      // whatever the offsets say, within [0, R]
     if (!p.offsets) { *first = 0; return p.R; }
     int a = __ldg(p.offsets + e), b = __ldg(p.offsets + e + 1);
@@ -223,52 +250,145 @@ __global__ void __launch_bounds__(kW4Threads, 2) w4_kernel(const W4Params p) {
     *first = a;
     return b - a;
   };
-  // Units of work of the experts before e: the same in every CTA.
-  for (int e = threadIdx.x; e < p.E; e += kW4Threads) {
+  // Chunks of up to 16 rows before expert e: the same in every CTA.
+  for (int e = threadIdx.x; e < p.E; e += kThreads) {
     int first;
-    s_units[e] = (rows_of(e, &first) + kMaxRows - 1) / kMaxRows;
+    s_chunks[e] = (rows_of(e, &first) + kMaxRows - 1) / kMaxRows;
   }
   __syncthreads();
   if (threadIdx.x < 32) {
     int sum = 0;
-    const int lane = threadIdx.x;
     for (int e0 = 0; e0 < p.E; e0 += 32) {
-      const int e = e0 + lane, v = e < p.E ? s_units[e] : 0;
+      const int e = e0 + lane, v = e < p.E ? s_chunks[e] : 0;
       int incl = v;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
         const int o = __shfl_up_sync(0xffffffffu, incl, off);
         if (lane >= off) incl += o;
       }
-      if (e < p.E) s_units[e] = sum + incl - v;
+      if (e < p.E) s_chunks[e] = sum + incl - v;
       sum += __shfl_sync(0xffffffffu, incl, 31);
     }
-    if (lane == 0) s_units[p.E] = sum;
+    if (lane == 0) s_chunks[p.E] = sum;
   }
   __syncthreads();
-  // Unit u: chunk of rows c, block of weight rows; a chunk's blocks follow one another.
-  const int64_t units = (int64_t)s_units[p.E] * blocks;
-  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-    const int c = (int)(u / blocks), m0 = (int)(u - (int64_t)c * blocks) * kUnitTiles;
-    int lo = 0, hi = p.E;                      // the expert e with s_units[e] <= c < s_units[e + 1]
+  // The (chunk, row of tiles) pairs are dealt out evenly: CTA b takes [first, last).
+  const int64_t total = (int64_t)s_chunks[p.E] * p.n_tiles;
+  const int64_t first = total * blockIdx.x / gridDim.x, last = total * (blockIdx.x + 1) / gridDim.x;
+  auto task_at = [&](int64_t at) {
+    Task w;
+    const int c = (int)(at / p.n_tiles);
+    w.m0 = (int)(at - (int64_t)c * p.n_tiles);
+    int lo = 0, hi = p.E;                      // the expert e with s_chunks[e] <= c < s_chunks[e + 1]
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (s_units[mid] <= c) lo = mid; else hi = mid;
+      if (s_chunks[mid] <= c) lo = mid; else hi = mid;
     }
-    int first;
-    const int rows = rows_of(lo, &first), chunks = (rows + kMaxRows - 1) / kMaxRows, i = c - s_units[lo];
-    const int a = (int)((int64_t)rows * i / chunks), cnt = (int)((int64_t)rows * (i + 1) / chunks) - a;
-    const int m1 = m0 + kUnitTiles < p.n_tiles ? m0 + kUnitTiles : p.n_tiles;
-    if (cnt <= 8) run_unit<T, 1, 4, SMALL, ZEROS>(p, lo, m0, m1, first + a, cnt, s_out);
-    else if (cnt <= 16) run_unit<T, 2, 4, SMALL, ZEROS>(p, lo, m0, m1, first + a, cnt, s_out);
-    else run_unit<T, 4, 2, SMALL, ZEROS>(p, lo, m0, m1, first + a, cnt, s_out);
+    w.e = lo;
+    int64_t left = last - at;
+    if (left > p.n_tiles - w.m0) left = p.n_tiles - w.m0;
+    const int steps = (int)((left + kM - 1) / kM);
+    w.m = (int)((left + steps - 1) / steps);   // even tasks
+    int r;
+    const int rows = rows_of(lo, &r), chunks = (rows + kMaxRows - 1) / kMaxRows, i = c - s_chunks[lo];
+    const int a = (int)((int64_t)rows * i / chunks);
+    w.r0 = r + a;
+    w.cnt = (int)((int64_t)rows * (i + 1) / chunks) - a;
+    return w;
+  };
+  const int k0 = (int)((int64_t)p.k_tiles * warp / kWarps), k1 = (int)((int64_t)p.k_tiles * (warp + 1) / kWarps);
+
+  griddep_wait();                              // x is there
+  griddep_launch_dependents();
+  // The copies run kStages - 1 steps ahead of the products, across tasks.
+  int64_t ahead_at = first;
+  int ahead_k = k0, ahead_slot = 0;
+  Task ahead;
+  if (first < last) ahead = task_at(first);
+  auto advance = [&]() {
+    if (ahead_at < last && k0 < k1) {
+      fill(p, ahead, ahead_k, ring + ahead_slot);
+      if (++ahead_k == k1) {
+        ahead_k = k0;
+        ahead_at += ahead.m;
+        if (ahead_at < last) ahead = task_at(ahead_at);
+      }
+    }
+    ahead_slot = ahead_slot + 1 == kStages ? 0 : ahead_slot + 1;
+    copies_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) advance();
+  int slot = 0;
+  auto run = [&](const Task& w, auto nt_tag) {
+    constexpr int NT = decltype(nt_tag)::value;
+    float sums[kM][NT][4];
+#pragma unroll
+    for (int m = 0; m < kM; ++m)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sums[m][nt][i] = 0.f;
+    const int g = lane >> 2, t = lane & 3;
+    const __half* rows[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+      rows[nt] = nt * 8 + g < w.cnt ? p.x + (size_t)(w.r0 + nt * 8 + g) * p.D + 8 * t : nullptr;
+    uint4 x[NT][2], next[NT][2];
+    load_x<NT>(p, rows, k0, next);
+#pragma unroll 1
+    for (int k = k0; k < k1; ++k) {
+      __syncwarp();                            // the slot that is filled next has been read by all lanes
+      advance();
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) { x[nt][0] = next[nt][0]; x[nt][1] = next[nt][1]; }
+      if (k + 1 < k1) load_x<NT>(p, rows, k + 1, next);
+      copies_wait<kStages - 1>();
+      __syncwarp();
+      multiply<T, NT, SMALL, ZEROS>(ring + slot, w.m, x, sums);
+      slot = slot + 1 == kStages ? 0 : slot + 1;
+    }
+    // The warps' sums meet in shared memory and are added in warp order.
+    float* mine = s_sums + warp * (kMaxRows * kSumStride);
+#pragma unroll
+    for (int m1 = 0; m1 < kM; m1 += kSumM) {
+      if (m1 >= w.m) break;
+#pragma unroll
+      for (int m = 0; m < kSumM; ++m)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            mine[(nt * 8 + 2 * t + (i & 1)) * kSumStride + m * 16 + g + 8 * (i >> 1)] = sums[m1 + m][nt][i];
+      __syncthreads();
+      const int width = (w.m - m1) * 16;
+      for (int o = threadIdx.x; o < w.cnt * kSumM * 16; o += kThreads) {
+        const int row = o / (kSumM * 16), n = o % (kSumM * 16), col = (w.m0 + m1) * 16 + n;
+        if (n >= width || col >= p.N) continue;
+        float v = 0.f;
+#pragma unroll
+        for (int q = 0; q < kWarps; ++q) v += s_sums[(q * kMaxRows + row) * kSumStride + n];
+        v = ldexpf(v, 24 + (p.row_exp ? __ldg(p.row_exp + w.r0 + row) : 0));
+        const size_t at = (size_t)(w.r0 + row) * p.N + col;
+        if (p.out_f32) static_cast<float*>(p.y)[at] = v;
+        else static_cast<T*>(p.y)[at] = from_float<T>(v);
+      }
+      __syncthreads();
+    }
+  };
+  for (int64_t at = first; at < last;) {
+    const Task w = task_at(at);
+    if (w.cnt <= 8) run(w, std::integral_constant<int, 1>{});
+    else run(w, std::integral_constant<int, 2>{});
+    at += w.m;
   }
+  copies_wait<0>();
   if (p.zero_rest && p.offsets) {              // rows of no expert
     int a = __ldg(p.offsets), b = __ldg(p.offsets + p.E);
     a = a < 0 ? 0 : a > p.R ? p.R : a;
     b = b < a ? a : b > p.R ? p.R : b;
     const int64_t rest = (int64_t)(p.R - (b - a)) * p.N;
-    for (int64_t i = (int64_t)blockIdx.x * kW4Threads + threadIdx.x; i < rest; i += (int64_t)gridDim.x * kW4Threads) {
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < rest; i += (int64_t)gridDim.x * kThreads) {
       int64_t r = i / p.N;
       const int64_t n = i - r * p.N;
       if (r >= a) r += b - a;
@@ -278,11 +398,37 @@ __global__ void __launch_bounds__(kW4Threads, 2) w4_kernel(const W4Params p) {
   }
 }
 
+// Workspace of a bf16 call: the rows in fp16, then their exponents.
+uint64_t rows_bytes(int64_t R, int64_t d) { return ((uint64_t)R * d * 2 + 255) & ~uint64_t(255); }
+
+template <typename T, bool SMALL, bool ZEROS>
+int launch_w4(const W4Params& p, const void* x, int sms, cudaStream_t s) {
+  constexpr size_t kSmem = kRingBytes<SMALL, ZEROS> + kSumBytes;
+  static_assert((kSmem + 4 * (kMaxExperts + 4) + 1024) * kCtasPerSm <= 227 * 1024, "shared memory of the resident CTAs");
+  static std::atomic<void*> seen[kMaxCachedDevices];
+  cudaError_t e = once_per_context(seen, [] {
+    return cudaFuncSetAttribute(w4_kernel<T, SMALL, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
+  });
+  if (e != cudaSuccess) return cuda_status(e);
+  if (p.row_exp) {
+    e = launch_pdl(w4_convert_kernel, dim3(p.R), dim3(kConvertThreads), 0, s, static_cast<const __nv_bfloat16*>(x),
+                   p.D, const_cast<__half*>(p.x), const_cast<int32_t*>(p.row_exp));
+    if (e != cudaSuccess) return cuda_status(e);
+  }
+  return cuda_status(launch_pdl(w4_kernel<T, SMALL, ZEROS>, dim3(kCtasPerSm * sms), dim3(kThreads), kSmem, s, p));
+}
+
 template <typename T>
-int run_w4(const W4Params& p, bool small, int sms, cudaStream_t s) {
-  auto kern = small ? (p.zeros ? w4_kernel<T, true, true> : w4_kernel<T, true, false>)
-                    : (p.zeros ? w4_kernel<T, false, true> : w4_kernel<T, false, false>);
-  return cuda_status(launch_pdl(kern, dim3(2 * sms), dim3(kW4Threads), 0, s, p));
+int run_w4(const W4Params& p, const void* x, bool small, int sms, cudaStream_t s) {
+  if (small) return p.zeros ? launch_w4<T, true, true>(p, x, sms, s) : launch_w4<T, true, false>(p, x, sms, s);
+  return p.zeros ? launch_w4<T, false, true>(p, x, sms, s) : launch_w4<T, false, false>(p, x, sms, s);
+}
+
+int check_w4(int32_t R, int32_t d, int32_t group_size, int32_t dtype) {
+  if (R < 0 || d < 1 || (group_size != 32 && group_size != 64 && group_size != 128) || d % group_size)
+    return MOE_ERR_INVALID_ARGUMENT;
+  if (dtype != MOE_F16 && dtype != MOE_BF16) return MOE_ERR_INVALID_ARGUMENT;
+  return d > INT32_MAX - 64 ? MOE_ERR_TOO_LARGE : MOE_OK;
 }
 
 }  // namespace
@@ -292,41 +438,53 @@ using namespace moe;
 
 extern "C" {
 
+MOE_API int moe_w4_workspace_size(int32_t num_rows, int32_t d, int32_t group_size, int32_t dtype, uint64_t* bytes) {
+  const int st = check_w4(num_rows, d, group_size, dtype);
+  if (st != MOE_OK) return st;
+  if (!bytes) return MOE_ERR_INVALID_ARGUMENT;
+  *bytes = dtype == MOE_BF16 ? rows_bytes(num_rows, d) + (uint64_t)num_rows * sizeof(int32_t) : 0;
+  return MOE_OK;
+}
+
 MOE_API int moe_w4_matvec(const void* x, const void* codes, const void* scales, const void* zeros,
                           const int32_t* offsets, int32_t num_rows, int32_t num_experts, int32_t n, int32_t d,
                           int32_t group_size, int32_t dtype, int32_t out_dtype, int32_t zero_other_rows, void* y,
-                          void* stream) {
-  if (num_rows < 0 || num_experts < 1 || n < 1 || d < 1) return MOE_ERR_INVALID_ARGUMENT;
-  if (group_size != 32 && group_size != 64 && group_size != 128) return MOE_ERR_INVALID_ARGUMENT;
-  if (d % group_size || (!offsets && num_experts != 1)) return MOE_ERR_INVALID_ARGUMENT;
-  if ((dtype != MOE_F16 && dtype != MOE_BF16) || (out_dtype != dtype && out_dtype != MOE_F32))
-    return MOE_ERR_INVALID_ARGUMENT;
-  if (num_experts > kMaxExperts || n > INT32_MAX - 64 || d > INT32_MAX - 64) return MOE_ERR_TOO_LARGE;
+                          void* workspace, uint64_t workspace_bytes, void* stream) {
+  int st = check_w4(num_rows, d, group_size, dtype);
+  if (st != MOE_OK) return st;
+  if (num_experts < 1 || n < 1 || (!offsets && num_experts != 1)) return MOE_ERR_INVALID_ARGUMENT;
+  if (out_dtype != dtype && out_dtype != MOE_F32) return MOE_ERR_INVALID_ARGUMENT;
+  if (num_experts > kMaxExperts || n > INT32_MAX - 64) return MOE_ERR_TOO_LARGE;
   if (num_rows == 0) return MOE_OK;
   if (!x || !codes || !scales || !y) return MOE_ERR_INVALID_ARGUMENT;
-  if (!aligned_to(x, 16) || !aligned_to(codes, 16) || !aligned_to(scales, 4) || !aligned_to(zeros, 2) ||
-      !aligned_to(offsets, 4) || !aligned_to(y, dtype_bytes(out_dtype)))
+  if (!aligned_to(x, 16) || !aligned_to(codes, 16) || !aligned_to(scales, 4) || !aligned_to(zeros, 4) ||
+      !aligned_to(offsets, 4) || !aligned_to(y, dtype_bytes(out_dtype)) || !aligned_to(workspace, 256))
     return MOE_ERR_MISALIGNED;
+  uint64_t need = 0;
+  moe_w4_workspace_size(num_rows, d, group_size, dtype, &need);
+  if (workspace_bytes < need || (need && !workspace)) return MOE_ERR_WORKSPACE_TOO_SMALL;
   int sms = 0;
-  const int st = require_device(&sms);
-  if (st != MOE_OK) return st;
+  if ((st = require_device(&sms)) != MOE_OK) return st;
   W4Params p;
-  p.x = x;
-  p.codes = static_cast<const uint4*>(codes);
-  p.scales = static_cast<const uint32_t*>(scales);
-  p.zeros = static_cast<const uint16_t*>(zeros);
-  p.offsets = offsets;
-  p.y = y;
   p.R = num_rows; p.N = n; p.D = d; p.E = num_experts;
   p.n_tiles = (n + 15) / 16;
   p.k_tiles = (d + kTileK - 1) / kTileK;
   p.groups = group_size == 32 ? 2 * p.k_tiles : d / group_size;   // whole tiles
   p.group_shift = group_size == 32 ? 5 : group_size == 64 ? 6 : 7;
+  p.x = static_cast<const __half*>(dtype == MOE_BF16 ? workspace : x);
+  p.row_exp = dtype == MOE_BF16 ? reinterpret_cast<const int32_t*>(static_cast<const uint8_t*>(workspace) +
+                                                                   rows_bytes(num_rows, d))
+                                : nullptr;
+  p.codes = static_cast<const uint4*>(codes);
+  p.scales = static_cast<const uint32_t*>(scales);
+  p.zeros = static_cast<const uint32_t*>(zeros);
+  p.offsets = offsets;
+  p.y = y;
   p.out_f32 = out_dtype == MOE_F32;
   p.zero_rest = zero_other_rows != 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == MOE_BF16 ? run_w4<__nv_bfloat16>(p, group_size == 32, sms, s)
-                           : run_w4<__half>(p, group_size == 32, sms, s);
+  return dtype == MOE_BF16 ? run_w4<__nv_bfloat16>(p, x, group_size == 32, sms, s)
+                           : run_w4<__half>(p, x, group_size == 32, sms, s);
 }
 
 }  // extern "C"

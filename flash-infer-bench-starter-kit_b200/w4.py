@@ -13,8 +13,12 @@ For inference only: there is no gradient.  The reference has no weights below
 
 from __future__ import annotations
 
+import ctypes
+import functools
+
 import torch
 
+from . import _lib
 from ._ops import DTYPES, call, check_tensor
 from .activation import swiglu
 from .tokens import _combine, dispatch, sort_tokens
@@ -95,12 +99,19 @@ class W4Weights:
         rows = n_tiles * _TILE_N
         c = _pad(codes, rows, k_tiles * _TILE_K // 2)
         q = torch.stack([c & 15, c >> 4], dim=2)
-        # (tile, row half, g; tile, h, t, word, pair, place) -> lane (g, t), word (h, word), nibble (place, pair, row half)
+        # (tile, row half, g; tile, half, t, word, pair, place) -> lane (g, t), word (half, word), byte (place, pair)
         q = q.view(n_tiles, 2, 8, k_tiles, 2, 4, 2, 2, 2).permute(0, 3, 2, 5, 4, 6, 8, 7, 1)
         self.codes[e].view(n_tiles, k_tiles, 8, 4, 2, 2, 2, 2).copy_(q[..., 0] | (q[..., 1] << 4))
         for out, t in ((self.scales, scales), (self.zeros, zeros)):
             if t is not None:
                 out[e].copy_(_pad(t, rows, groups).view(n_tiles, 2, 8, groups).permute(0, 3, 2, 1))
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(rows, d, group_size, dtype):
+    n = ctypes.c_uint64(0)
+    _lib.check(_lib.load().moe_w4_workspace_size(rows, d, group_size, dtype, ctypes.byref(n)), "moe_w4_workspace_size")
+    return int(n.value)
 
 
 def w4_matvec(x: torch.Tensor, weights: W4Weights, offsets: torch.Tensor | None = None,
@@ -110,7 +121,7 @@ def w4_matvec(x: torch.Tensor, weights: W4Weights, offsets: torch.Tensor | None 
 
     ``x`` [R, D] has the weights' type; ``offsets`` int32 [E + 1] as ``sort_tokens`` gives them, None for a
     single matrix.  Rows outside ``[offsets[0], offsets[E])`` are zero in a new result and left as they
-    were in a given ``out``.  The weights of each expert with rows are read once for up to 32 rows, so
+    were in a given ``out``.  The weights of each expert with rows are read once for up to 16 rows, so
     this is the product for decode batches; prefill batches want a GEMM."""
     if not isinstance(weights, W4Weights):
         raise TypeError("weights must be W4Weights")
@@ -134,8 +145,10 @@ def w4_matvec(x: torch.Tensor, weights: W4Weights, offsets: torch.Tensor | None 
         check_tensor("out", out, (x.dtype, torch.float32) if out_dtype is None else (out_dtype,), (R, weights.n), dev)
     if x.data_ptr() % 16:
         x = x.clone()
+    need = _workspace_bytes(R, weights.d, weights.group_size, DTYPES[x.dtype])
+    workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     call("moe_w4_matvec", dev, x, weights.codes, weights.scales, weights.zeros, offsets, R, weights.num_experts,
-         weights.n, weights.d, weights.group_size, DTYPES[x.dtype], DTYPES[out.dtype], int(fresh), out)
+         weights.n, weights.d, weights.group_size, DTYPES[x.dtype], DTYPES[out.dtype], int(fresh), out, workspace, need)
     return out
 
 

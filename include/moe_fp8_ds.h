@@ -319,17 +319,20 @@ MOE_API int moe_swiglu_backward(const void* grad_y, const void* codes, const flo
  * [R, n] has that type or fp32 (out_dtype).  Sums are fp32, rounded once.
  * group_size is 32, 64 or 128 and divides d.  Layout, with N = n rounded up to 16 and
  * D = d rounded up to 64 (all padding zero): codes [E][N / 16][D / 64][32 lanes][16
- * bytes]; lane 4 * g + t holds, in 32-bit word j, columns c = 32 * (j / 2) + 8 * t +
- * 4 * (j % 2) + {0, 1, 2, 3} of rows g and g + 8 as nibbles 0, 4 = (g; c, c + 1),
- * 1, 5 = (g + 8; c, c + 1), 2, 6 = (g; c + 2, c + 3), 3, 7 = (g + 8; c + 2, c + 3);
- * scales [E][N / 16][D / group_size][8][2] (rows g and g + 8 of a tile together);
- * zeros uint8, laid out as the scales, or NULL: 8.  Rows of x outside
- * [offsets[0], offsets[E]) get zeros when zero_other_rows is set, else their y is left as
- * it was.  num_experts <= 1024.                                               */
+ * bytes]; lane 4 * g + t holds, in bytes 0 to 3 of its 32-bit word j, columns 32 * (j / 2) +
+ * 8 * t + 4 * (j % 2) + {0, 2, 1, 3} of row g (low half) and of row g + 8 (high half); scales
+ * [E][N / 16][D / group_size][8][2] (rows g and g + 8 of a tile together); zeros uint8,
+ * laid out as the scales, or NULL: 8.  Rows of x outside [offsets[0], offsets[E]) get
+ * zeros when zero_other_rows is set, else their y is left as it was.  bf16 rows are
+ * scaled by a power of two each into fp16 in the workspace (moe_w4_workspace_size bytes, 0
+ * for fp16; 256-byte aligned, any contents, not shared by calls that may overlap):
+ * values more than 2^28 below the row's largest are off by at most 2^-39 of that,
+ * others by nothing.  x is 16-byte aligned.  num_experts <= 1024.             */
+MOE_API int moe_w4_workspace_size(int32_t num_rows, int32_t d, int32_t group_size, int32_t dtype, uint64_t* bytes);
 MOE_API int moe_w4_matvec(const void* x, const void* codes, const void* scales, const void* zeros,
                           const int32_t* offsets, int32_t num_rows, int32_t num_experts, int32_t n, int32_t d,
                           int32_t group_size, int32_t dtype, int32_t out_dtype, int32_t zero_other_rows, void* y,
-                          void* stream);
+                          void* workspace, uint64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -3,6 +3,7 @@ before anything is launched."""
 
 from __future__ import annotations
 
+import ctypes
 import sys
 
 import pytest
@@ -72,15 +73,21 @@ def test_swiglu_and_w4_entries_check_their_arguments(pkg):
     mv = lib.moe_w4_matvec
 
     def call(x=p, codes=p, scales=p, zeros=None, offsets=p, R=4, E=2, n=16, d=128, group=64, dt=L.MOE_BF16,
-             out=L.MOE_BF16, y=p):
-        return mv(x, codes, scales, zeros, offsets, R, E, n, d, group, dt, out, 0, y, None)
+             out=L.MOE_BF16, y=p, ws=256, nbytes=1 << 20):
+        return mv(x, codes, scales, zeros, offsets, R, E, n, d, group, dt, out, 0, y, ws, nbytes, None)
     assert call(R=-1) == call(E=0) == call(n=0) == call(d=0) == bad
     assert call(group=16) == call(group=256) == call(d=96) == bad
+    size = lib.moe_w4_workspace_size
+    assert size(4, 96, 64, L.MOE_F16, ctypes.byref(ctypes.c_uint64())) == bad
+    assert size(4, 128, 64, L.MOE_F32, ctypes.byref(ctypes.c_uint64())) == bad
+    assert size(4, 128, 64, L.MOE_F16, None) == bad
     assert call(offsets=None) == bad
     assert call(dt=L.MOE_F32) == call(out=L.MOE_F16) == bad
     assert call(codes=None) == call(x=None) == call(scales=None) == call(y=None) == bad
     assert call(E=1025) == big
-    assert call(x=p + 2) == call(codes=p + 8) == call(scales=p + 2) == call(zeros=p + 1) == call(y=p + 1) == odd
+    assert call(x=p + 2) == call(codes=p + 8) == call(scales=p + 2) == call(zeros=p + 2) == call(y=p + 1) == odd
+    assert call(ws=128) == odd
+    assert call(ws=None) == call(nbytes=4 * 128 * 2) == L.MOE_ERR_WORKSPACE_TOO_SMALL
     assert call(R=0, x=None, y=None) == L.MOE_OK
 
 
@@ -136,10 +143,10 @@ def test_w4_layout_is_the_documented_one(N, D, group, zero_points, pkg):
                 row, t = lane // 4, lane % 4
                 for j in range(4):
                     c = kt * 64 + 32 * (j // 2) + 8 * t + 4 * (j % 2)
-                    for nib, (r, k) in {0: (0, 0), 4: (0, 1), 1: (8, 0), 5: (8, 1), 2: (0, 2), 6: (0, 3), 3: (8, 2),
-                                        7: (8, 3)}.items():
+                    for nib in range(8):
                         for e in range(E):
-                            got[e, tile * 16 + row + r, c + k] = (int(words[e, tile, kt, lane, j]) >> (4 * nib)) & 15
+                            got[e, tile * 16 + row + 8 * (nib % 2), c + (0, 2, 1, 3)[nib // 2]] = \
+                                (int(words[e, tile, kt, lane, j]) >> (4 * nib)) & 15
     want = torch.zeros_like(got)
     want[:, :N, 0:D:2], want[:, :N, 1:D:2] = codes & 15, codes >> 4
     assert torch.equal(got, want)
