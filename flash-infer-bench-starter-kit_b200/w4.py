@@ -24,7 +24,6 @@ from .activation import swiglu
 from .tokens import _combine, dispatch, sort_tokens
 
 GROUP_SIZES = (32, 64, 128)
-_TILE_N, _TILE_K = 16, 64
 
 
 def quantize_w4(w: torch.Tensor, group_size: int, zero_points: bool = False, dtype: torch.dtype = torch.bfloat16):
@@ -46,10 +45,6 @@ def quantize_w4(w: torch.Tensor, group_size: int, zero_points: bool = False, dty
     q = (torch.round(v / s.unsqueeze(-1)) + zeros.unsqueeze(-1)).clamp(0, 15).to(torch.uint8).flatten(-2)
     codes = q[..., 0::2] | (q[..., 1::2] << 4)
     return codes, scales, zeros.to(torch.uint8) if zero_points else None
-
-
-def _pad(t, rows, cols):
-    return torch.nn.functional.pad(t, (0, cols - t.shape[1], 0, rows - t.shape[0]))
 
 
 class W4Weights:
@@ -83,34 +78,27 @@ class W4Weights:
         for name, t in (("scales", scales), ("zeros", zeros)):
             if t is not None and t.shape != (E, N, D // group_size):
                 raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {(E, N, D // group_size)}")
-        if zeros is not None and zeros.numel() and int(zeros.max()) > 15:
+        if not codes.is_cuda:
+            raise ValueError("codes, scales and zeros must be CUDA tensors (no CPU path)")
+        if zeros is not None and int(zeros.max()) > 15:
             raise ValueError("zeros must be 0 to 15")
         self.num_experts, self.n, self.d, self.group_size = E, N, D, group_size
-        self.dtype, self.device = scales.dtype, codes.device
-        n_tiles, k_tiles = -(-N // _TILE_N), -(-D // _TILE_K)
-        groups = k_tiles * _TILE_K // group_size
-        self.codes = torch.empty(E, n_tiles, k_tiles, 32, 16, dtype=torch.uint8, device=codes.device)
-        self.scales = torch.empty(E, n_tiles, groups, 8, 2, dtype=scales.dtype, device=codes.device)
-        self.zeros = torch.empty_like(self.scales, dtype=torch.uint8) if zeros is not None else None
-        for e in range(E):
-            self._lay_out(e, codes[e], scales[e], zeros[e] if zeros is not None else None, n_tiles, k_tiles, groups)
-
-    def _lay_out(self, e, codes, scales, zeros, n_tiles, k_tiles, groups):
-        rows = n_tiles * _TILE_N
-        c = _pad(codes, rows, k_tiles * _TILE_K // 2)
-        q = torch.stack([c & 15, c >> 4], dim=2)
-        # (tile, row half, g; tile, half, t, word, pair, place) -> lane (g, t), word (half, word), byte (place, pair)
-        q = q.view(n_tiles, 2, 8, k_tiles, 2, 4, 2, 2, 2).permute(0, 3, 2, 5, 4, 6, 8, 7, 1)
-        self.codes[e].view(n_tiles, k_tiles, 8, 4, 2, 2, 2, 2).copy_(q[..., 0] | (q[..., 1] << 4))
-        for out, t in ((self.scales, scales), (self.zeros, zeros)):
-            if t is not None:
-                out[e].copy_(_pad(t, rows, groups).view(n_tiles, 2, 8, groups).permute(0, 3, 2, 1))
+        self.dtype, self.device, self.with_zeros = scales.dtype, codes.device, zeros is not None
+        nbytes = ctypes.c_uint64(0)
+        _lib.check(_lib.load().moe_w4_layout_size(E, N, D, group_size, int(self.with_zeros), ctypes.byref(nbytes)),
+                   "moe_w4_layout_size")
+        self.layout = torch.empty(nbytes.value, dtype=torch.uint8, device=self.device)
+        codes, scales = codes.contiguous(), scales.contiguous()
+        zeros = zeros.contiguous() if zeros is not None else None
+        if codes.data_ptr() % 4:
+            codes = codes.clone()
+        call("moe_w4_lay_out", self.device, codes, scales, zeros, E, N, D, group_size, self.layout)
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(rows, d, group_size, dtype):
+def _workspace_bytes(rows, d, dtype):
     n = ctypes.c_uint64(0)
-    _lib.check(_lib.load().moe_w4_workspace_size(rows, d, group_size, dtype, ctypes.byref(n)), "moe_w4_workspace_size")
+    _lib.check(_lib.load().moe_w4_workspace_size(rows, d, dtype, ctypes.byref(n)), "moe_w4_workspace_size")
     return int(n.value)
 
 
@@ -145,10 +133,11 @@ def w4_matvec(x: torch.Tensor, weights: W4Weights, offsets: torch.Tensor | None 
         check_tensor("out", out, (x.dtype, torch.float32) if out_dtype is None else (out_dtype,), (R, weights.n), dev)
     if x.data_ptr() % 16:
         x = x.clone()
-    need = _workspace_bytes(R, weights.d, weights.group_size, DTYPES[x.dtype])
+    need = _workspace_bytes(R, weights.d, DTYPES[x.dtype])
     workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    call("moe_w4_matvec", dev, x, weights.codes, weights.scales, weights.zeros, offsets, R, weights.num_experts,
-         weights.n, weights.d, weights.group_size, DTYPES[x.dtype], DTYPES[out.dtype], int(fresh), out, workspace, need)
+    call("moe_w4_matvec", dev, x, weights.layout, offsets, R, weights.num_experts, weights.n, weights.d,
+         weights.group_size, int(weights.with_zeros), DTYPES[x.dtype], DTYPES[out.dtype], int(fresh), out, workspace,
+         need)
     return out
 
 

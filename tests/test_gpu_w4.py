@@ -73,6 +73,87 @@ def test_w4_matvec(E, N, D, group, rows, zeros, dtype, pkg, cuda_dev):
         assert torch.equal(pkg.w4_matvec(x, single), y)
 
 
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("N,D,group", [(16, 128, 64), (20, 96, 32), (33, 256, 128), (1, 32, 32), (48, 192, 64)])
+def test_layout_is_the_documented_one(N, D, group, zeros, pkg, cuda_dev):
+    """Every code, scale and zero point is where the header says, padding is zero."""
+    E = 2
+    codes, scales, z = make(E, N, D, group, zeros, torch.float16, cuda_dev, N + D)
+    w = pkg.W4Weights(codes, scales, z, group_size=group)
+    n16, steps, groups = -(-N // 16), -(-D // 128), 128 // group
+    rec = w.layout.cpu().view(E, n16, steps, -1)
+    assert rec.shape[-1] == 1024 + groups * (48 if zeros else 32)
+    words = rec[..., :1024].contiguous().view(E, n16, steps, 2, 32, 16)
+    got = torch.zeros(E, n16 * 16, steps * 128, dtype=torch.uint8)
+    for lane in range(32):
+        row, t = lane // 4, lane % 4
+        for j in range(4):
+            for i, k in enumerate((0, 2, 1, 3)):
+                byte = words[:, :, :, :, lane, 4 * j + i]                      # [E, n16, steps, 2]
+                c = 32 * (j // 2) + 8 * t + 4 * (j % 2) + k
+                got[:, row::16, c::64] = (byte & 15).flatten(2)
+                got[:, row + 8::16, c::64] = (byte >> 4).flatten(2)
+    want = torch.zeros_like(got)
+    want[:, :N, 0:D:2], want[:, :N, 1:D:2] = (codes & 15).cpu(), (codes >> 4).cpu()
+    assert torch.equal(got, want)
+    tail = rec[..., 1024:1024 + 32 * groups].contiguous().view(torch.float16)
+    for part, plain in ((tail, scales), (rec[..., 1024 + 32 * groups:], z)):
+        if plain is None:
+            assert part.numel() == 0
+            continue
+        full = torch.zeros(E, n16 * 16, steps * groups, dtype=plain.dtype)
+        full[:, :N, :D // group] = plain.cpu()
+        part = part.reshape(E, n16, steps, groups, 8, 2).permute(0, 1, 5, 4, 2, 3)
+        assert torch.equal(part.reshape(E, n16 * 16, -1), full)
+
+
+def test_pruned_weights_and_small_values_are_exact(pkg, cuda_dev):
+    """Codes equal to their zero points give exact zeros, and a value far below its row's largest still counts
+    where the largest has no weight."""
+    torch.manual_seed(0)
+    N, D = 40, 256
+    z = torch.randint(0, 16, (1, N, D // 32), device=cuda_dev, dtype=torch.uint8)
+    q = z.repeat_interleave(32, -1)
+    s = torch.rand(1, N, D // 32, device=cuda_dev).bfloat16() + 1
+    x = torch.randn(3, D, device=cuda_dev).bfloat16() * 1000
+    off = torch.tensor([0, 3], dtype=torch.int32, device=cuda_dev)
+    w = pkg.W4Weights(q[..., 0::2] | q[..., 1::2] << 4, s, z, group_size=32)
+    assert not bool(pkg.w4_matvec(x, w, off).any())
+    w = pkg.W4Weights(torch.full((1, N, D // 2), 0x88, dtype=torch.uint8, device=cuda_dev), s, group_size=32)
+    assert not bool(pkg.w4_matvec(x, w, off).any())
+    codes = torch.full((1, N, D // 2), 0x88, dtype=torch.uint8, device=cuda_dev)
+    codes[0, :, 5] = 0x89                                       # column 10 counts once, column 11 not at all
+    w = pkg.W4Weights(codes, s, group_size=32)
+    x = torch.zeros(1, D, device=cuda_dev).bfloat16()
+    x[0, 10], x[0, 11] = 1.5 * 2.0 ** -20, 2.0 ** 8
+    y = pkg.w4_matvec(x, w, off[:1].repeat(2) + torch.tensor([0, 1], device=cuda_dev, dtype=torch.int32))
+    assert torch.equal(y[0], (s[0, :, 0].float() * 1.5 * 2.0 ** -20).bfloat16())
+
+
+@pytest.mark.parametrize("size", [2.0 ** -126, 2.0 ** -60, 2.0 ** 60, 2.0 ** 120])
+def test_rows_of_any_size(size, pkg, cuda_dev):
+    """bf16 rows at the ends of the type's range, next to ordinary ones."""
+    codes, scales, z = make(1, 33, 128, 64, True, torch.bfloat16, cuda_dev, 3)
+    w = pkg.W4Weights(codes, scales, z, group_size=64)
+    x = torch.randn(4, 128, device=cuda_dev).bfloat16()
+    x[1] *= size
+    y = pkg.w4_matvec(x, w, out_dtype=torch.float32)
+    check(y, x, dense(codes, scales, z, 64), [0, 4], torch.float32, 128)
+
+
+def test_infinities(pkg, cuda_dev):
+    codes, scales, z = make(1, 64, 128, 64, False, torch.bfloat16, cuda_dev, 4)
+    w = pkg.W4Weights(codes, scales, z, group_size=64)
+    x = torch.randn(3, 128, device=cuda_dev).bfloat16()
+    clean = pkg.w4_matvec(x, w)
+    x[1, 7] = float("inf")
+    y = pkg.w4_matvec(x, w)
+    W = dense(codes, scales, z, 64)[0, :, 7]
+    want = torch.where(W == 0, float("nan"), torch.sign(W) * float("inf")).bfloat16()
+    assert torch.equal(y[1].nan_to_num(7.0), want.nan_to_num(7.0)) and torch.equal(y[0], clean[0])
+    assert torch.equal(y[2], clean[2])
+
+
 def test_rows_of_no_expert(pkg, cuda_dev):
     """Zero in a new result, untouched in a given one; a NaN row spoils no other."""
     codes, scales, _ = make(3, 70, 128, 64, False, torch.bfloat16, cuda_dev, 0)
@@ -213,6 +294,12 @@ def test_refusals(pkg, cuda_dev):
                           ((x, w, off), {"out": x}, ValueError), ((x, w, off.cpu()), {}, ValueError)]:
         with pytest.raises(err):
             pkg.w4_matvec(*args, **kw)
+    for bad in ((codes, scales[0]), (codes[:, :, :8], scales), (codes, scales, torch.full(
+            scales.shape, 16, dtype=torch.uint8, device=cuda_dev)), (codes, scales.cpu())):
+        with pytest.raises(ValueError):
+            pkg.W4Weights(*bad, group_size=32)
+    with pytest.raises(ValueError):
+        pkg.W4Weights(codes, scales, group_size=64)
     ids = torch.zeros(4, 1, dtype=torch.int32, device=cuda_dev)
     with pytest.raises(ValueError):
         pkg.moe_w4(x, ids, torch.zeros(4, 1, device=cuda_dev), w, w)
