@@ -16,14 +16,15 @@
 // tcgen05 would want the decoded weights in shared memory or TMEM and 128-row tiles; a
 // decode batch has too few rows of x for that to pay.)
 //
-// fp16 rows of x are the other operand as they are.  bf16 rows are first brought
-// to fp16 by a power of two for each row that puts its largest magnitude into
-// [2^14, 2^15): exact for values down to 2^-28 of the largest, below that off by at
-// most 2^-39 of it.  (Next to an infinity or a NaN the finite values vanish, as they
-// do in the sum.)
+// bf16 rows of x are brought to fp16 by a power of two for each row that puts its
+// largest magnitude into [2^14, 2^15): exact for values down to 2^-28 of the largest,
+// below that off by at most 2^-39 of it.  (Next to an infinity or a NaN the finite
+// values vanish, as they do in the sum.)
 //
-// Layout (made once, by moe_w4_lay_out): records of 16 rows x 128 columns,
-// [E][N / 16][D / 128][record], each one piece of memory that a warp streams:
+// Layout (made once, by moe_w4_lay_out): records of 16 rows x 128 columns, in the
+// order in which a CTA streams them, so that what it takes at a time is one or two
+// pieces of memory: [E][groups of 8 rows of records][stages of 4 columns of records]
+// [8][4][record], where the last group and the last stage may be smaller.  A record is
 //   two 16 x 64 tiles of codes in the order in which a warp's lanes take them, 16
 //   bytes a lane.  With lane = 4 * g + t, 32-bit word j holds columns c = 32 * (j / 2) +
 //   8 * t + 4 * (j % 2) + {0, 2, 1, 3} in its bytes 0 to 3, row g in the low half of a
@@ -31,35 +32,43 @@
 //   bytes for each 32 columns;
 //   the record's scales [128 / G][8][2] (rows g, g + 8 together), then, if there are any,
 //   its zero points likewise.
+#include <type_traits>
+
 #include "rows.cuh"
 
 namespace moe {
 namespace {
 
-constexpr int kWarps = 8;                 // of a CTA
-constexpr int kThreads = kWarps * 32;
-constexpr int kCtasPerSm = 2;
-constexpr int kM = 4;                     // rows of records a warp works on together
-constexpr int kMaxRows = 16;              // rows of x in a task
-constexpr int kStages = 2;                // of a warp's ring of records
 constexpr int kStepK = 128;               // columns of a record
+constexpr int kSplit = 4;                 // warps along the columns: a stage holds 4 steps
+constexpr int kGroupsM = 4;               // groups of warps along the rows of tiles
+constexpr int kM = 2;                     // rows of tiles (of records) of a warp
+constexpr int kTaskM = kM * kGroupsM;     // of a task
+constexpr int kConsumers = kSplit * kGroupsM;       // warps that multiply; one more copies
+constexpr int kThreads = (kConsumers + 1) * 32;
+constexpr int kStages = 3;
+constexpr int kMaxRows = 24;              // rows of x in a task
 constexpr int kMaxExperts = 1024;
-constexpr int kSumM = 2;                  // rows of records whose sums are joined at a time
-constexpr int kSumStride = kSumM * 16 + 4;   // of the sums in shared memory: a warp's stores hit 32 banks
-constexpr size_t kSumBytes = sizeof(float) * kWarps * kMaxRows * kSumStride;
+constexpr int kStageK = kSplit * kStepK;  // columns of a stage
+constexpr int kRowPiece = kStageK * 2;    // bytes of a row of x in a stage
+constexpr int kSumStride = kM * 16 + 4;   // of the sums in shared memory: a warp's stores hit 32 banks
+constexpr size_t kSumBytes = sizeof(float) * kConsumers * 8 * kSumStride;
 
 // Bytes of a record with groups of G columns.
 __host__ __device__ constexpr int record_bytes(int G, bool zeros) { return 1024 + kStepK / G * (zeros ? 48 : 32); }
 
 struct W4Params {
-  const __half* x;         // [R, D]
-  const int32_t* row_exp;  // [R]: the exponent taken out of a bf16 row, or null: 0
-  const uint8_t* records;  // [E][n_tiles][k_steps][record]
+  const uint8_t* x;        // [stages][R][kRowPiece]
+  const int32_t* row_exp;  // [R]: the exponent taken out of a row
+  const uint8_t* records;  // as above
   const int32_t* offsets;  // [E + 1], or null: one matrix for all rows
   void* y;
-  int R, N, D, E, n_tiles, k_steps, k_split;
+  int R, N, E, n_tiles, k_steps, stages;
   int out_f32, zero_rest;
 };
+
+// Set when a wait gave up; read and cleared by moe_w4_read_device_error.
+__device__ int g_w4_error;
 
 // --------------------------------------------------------------------------
 // The layout: a thread makes 16 bytes.  Padding (rows behind N, columns behind D) is
@@ -74,10 +83,14 @@ w4_lay_out_kernel(const uint8_t* __restrict__ codes, const uint16_t* __restrict_
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= pieces) return;
   const int groups = kStepK / G, per_record = record_bytes(G, zeros != nullptr) / 16;
-  const int64_t record = at / per_record, tile = record / k_steps;
-  const int piece = (int)(at - record * per_record), step = (int)(record - tile * k_steps);
-  const int64_t e = tile / n_tiles;
-  const int row0 = (int)(tile - e * n_tiles) * 16;
+  const int64_t record = at / per_record, per_expert = (int64_t)n_tiles * k_steps, e = record / per_expert;
+  const int piece = (int)(at - record * per_record);
+  const int in_expert = (int)(record - e * per_expert), group = in_expert / (kTaskM * k_steps);
+  const int in_group = in_expert - group * (kTaskM * k_steps);
+  const int tiles = n_tiles - group * kTaskM < kTaskM ? n_tiles - group * kTaskM : kTaskM;
+  const int stage = in_group / (tiles * kSplit), in_stage = in_group - stage * (tiles * kSplit);
+  const int steps = k_steps - stage * kSplit < kSplit ? k_steps - stage * kSplit : kSplit;
+  const int row0 = (group * kTaskM + in_stage / steps) * 16, step = stage * kSplit + in_stage % steps;
   union { uint4 v; uint8_t b[16]; uint16_t h[8]; } o;
   o.v = make_uint4(0, 0, 0, 0);
   if (piece < 64) {
@@ -110,9 +123,9 @@ w4_lay_out_kernel(const uint8_t* __restrict__ codes, const uint16_t* __restrict_
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       if (i >= n) break;
-      const int v = first + i, group = step * groups + v / 16, row = row0 + (v & 15) / 2 + 8 * (v & 1);
-      if (row >= N || group * G >= D) continue;
-      const size_t src = ((size_t)e * N + row) * (D / G) + group;
+      const int v = first + i, of = step * groups + v / 16, row = row0 + (v & 15) / 2 + 8 * (v & 1);
+      if (row >= N || of * G >= D) continue;
+      const size_t src = ((size_t)e * N + row) * (D / G) + of;
       if (is_zeros) o.b[i] = zeros[src];
       else o.h[i] = scales[src];
     }
@@ -120,50 +133,6 @@ w4_lay_out_kernel(const uint8_t* __restrict__ codes, const uint16_t* __restrict_
   *reinterpret_cast<uint4*>(out + at * 16) = o.v;
 }
 
-// --------------------------------------------------------------------------
-// bf16 rows to fp16: a CTA takes a row, finds its largest magnitude and scales by
-// 2^-exp.  Reads and writes R * D * 2 bytes, a few microseconds of latency.
-// --------------------------------------------------------------------------
-constexpr int kConvertThreads = 256;
-
-__global__ void __launch_bounds__(kConvertThreads)
-w4_convert_kernel(const __nv_bfloat16* __restrict__ x, int D, __half* __restrict__ out, int32_t* __restrict__ row_exp) {
-  __shared__ float s_max[kConvertThreads / 32];
-  griddep_wait();
-  griddep_launch_dependents();
-  const size_t base = (size_t)blockIdx.x * D;
-  float amax = 0.f;
-  for (int i = threadIdx.x * 8; i < D; i += kConvertThreads * 8) {   // D is a multiple of 32
-    const Pack<__nv_bfloat16, 8> v = load_cached<__nv_bfloat16, 8>(x + base + i);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float a = fabsf(to_float(v.v[j]));
-      amax = a < INFINITY ? fmaxf(amax, a) : INFINITY;
-    }
-  }
-#pragma unroll
-  for (int off = 16; off; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = amax;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kConvertThreads / 32; ++i) amax = fmaxf(amax, s_max[i]);
-  // amax * 2^-exp in [2^14, 2^15), as far as 2^-exp is a normal number
-  int exp = (int)((__float_as_uint(amax) >> 23) & 0xff) - 127 - 14;
-  exp = exp < -120 ? -120 : exp;
-  const float down = __uint_as_float((uint32_t)(127 - exp) << 23);
-  for (int i = threadIdx.x * 8; i < D; i += kConvertThreads * 8) {
-    const Pack<__nv_bfloat16, 8> v = load_cached<__nv_bfloat16, 8>(x + base + i);
-    Pack<__half, 8> h;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) h.v[j] = __float2half_rn(to_float(v.v[j]) * down);
-    store_wide<__half, 8>(out + base + i, h);
-  }
-  if (threadIdx.x == 0) row_exp[blockIdx.x] = exp;
-}
-
-// --------------------------------------------------------------------------
-// The product.
-// --------------------------------------------------------------------------
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                         uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -176,13 +145,74 @@ __device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {   // sub
   return d;
 }
 
-// Asynchronous copies to shared memory.
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// --------------------------------------------------------------------------
+// Rows of x for the product: a CTA takes 8 rows, finds the largest magnitude of each
+// (bf16) and writes them in fp16 by stages of 512 columns, zeros behind D; 16-byte pieces 4
+// apart change places in odd rows, so that a warp's reads of 8 rows hit 32 banks.
+// Reads and writes R * D * 2 bytes, out of and into L2: latency.
+// --------------------------------------------------------------------------
+constexpr int kRowsThreads = 512;
+
+template <typename T>
+__global__ void __launch_bounds__(kRowsThreads)
+w4_rows_kernel(const T* __restrict__ x, int R, int D, int stages, uint8_t* __restrict__ out,
+               int32_t* __restrict__ row_exp) {
+  constexpr int kWarps = kRowsThreads / 32;
+  constexpr bool kScaled = !std::is_same<T, __half>::value;
+  __shared__ float s_max[kWarps];
+  griddep_wait();
+  griddep_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // warps w and w + 8: the two halves of row w
+  const int row = blockIdx.x * 8 + (warp & 7);
+  int exp = 0;
+  if constexpr (kScaled) {
+    float amax = 0.f;
+    if (row < R)
+#pragma unroll 4
+      for (int i = (warp >> 3) * 256 + lane * 8; i < D; i += 512) {   // D is a multiple of 32
+        const Pack<T, 8> v = load_cached<T, 8>(x + (size_t)row * D + i);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float a = fabsf(to_float(v.v[j]));
+          amax = a < INFINITY ? fmaxf(amax, a) : INFINITY;
+        }
+      }
+#pragma unroll
+    for (int off = 16; off; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+    if (lane == 0) s_max[warp] = amax;
+    __syncthreads();
+    amax = fmaxf(s_max[warp & 7], s_max[(warp & 7) + 8]);
+    // amax * 2^-exp in [2^14, 2^15), as far as 2^-exp is a normal number
+    exp = (int)((__float_as_uint(amax) >> 23) & 0xff) - 127 - 14;
+    exp = exp < -120 ? -120 : exp;
+  }
+  if (row >= R) return;
+  const float down = __uint_as_float((uint32_t)(127 - exp) << 23);
+#pragma unroll 4
+  for (int i = (warp >> 3) * 256 + lane * 8; i < stages * kStageK; i += 512) {
+    Pack<__half, 8> o = zero_pack<__half, 8>();
+    if (i < D) {
+      const Pack<T, 8> v = load_cached<T, 8>(x + (size_t)row * D + i);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        o.v[j] = kScaled ? __float2half_rn(to_float(v.v[j]) * down) : from_float<__half>(to_float(v.v[j]));
+    }
+    const int stage = i / kStageK, piece = (i % kStageK / 8) ^ ((row & 1) << 2);
+    store_wide<__half, 8>(reinterpret_cast<__half*>(out + ((size_t)stage * R + row) * kRowPiece) + piece * 8, o);
+  }
+  if (warp < 8 && lane == 0) row_exp[row] = exp;
 }
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// --------------------------------------------------------------------------
+// The product.
+// --------------------------------------------------------------------------
+// One piece of memory into shared memory, counted by an mbarrier; 16-byte aligned.
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
 
 template <typename T> __device__ __forceinline__ float2 pair_of(uint32_t v);
 template <> __device__ __forceinline__ float2 pair_of<__nv_bfloat16>(uint32_t v) {
@@ -198,36 +228,93 @@ struct Task {
   int c, e, m0, m, r0, cnt;
 };
 
-// A step: kM records of 128 columns (`m_here` of them are there) times NT * 8 rows of x,
-// half a record at a time so that the next half's x can be on its way.
-template <typename T, int NT, int G, bool ZEROS>
-struct Step {
-  static constexpr int kRecord = record_bytes(G, ZEROS);
-  static constexpr int kGroups = G == 32 ? 2 : 1;        // in half a record
+// The tasks of a CTA.  The (chunk, row of tiles) pairs are dealt out evenly: CTA b takes the
+// pairs [total * b / CTAs, total * (b + 1) / CTAs), in even tasks of at most kTaskM tiles.
+struct Tasks {
+  const W4Params* p;
+  const int* chunks_before;   // [E + 1]
+  int last_c, last_m;
 
-  // A lane's share of half a record's columns of x.
-  static __device__ __forceinline__ void load_x(const __half* const (&rows)[NT], int col, int D, uint4 (&x)[NT][2]) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const bool in = col + 32 * h < D;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        x[nt][h] = in ? __ldg(reinterpret_cast<const uint4*>(rows[nt] + col + 32 * h)) : make_uint4(0, 0, 0, 0);
-    }
+  // Rows of expert e, whatever the offsets say within [0, R].
+  static __device__ __forceinline__ int rows_of(const W4Params& p, int e, int* first) {
+    if (!p.offsets) { *first = 0; return p.R; }
+    int a = __ldg(p.offsets + e), b = __ldg(p.offsets + e + 1);
+    a = a < 0 ? 0 : a > p.R ? p.R : a;
+    b = b < a ? a : b > p.R ? p.R : b;
+    *first = a;
+    return b - a;
   }
+  __device__ __forceinline__ Task begin() {
+    const int64_t total = (int64_t)chunks_before[p->E] * p->n_tiles;
+    const int64_t first = total * blockIdx.x / gridDim.x, last = total * (blockIdx.x + 1) / gridDim.x;
+    last_c = (int)(last / p->n_tiles);
+    last_m = (int)(last - (int64_t)last_c * p->n_tiles);
+    Task w;
+    w.c = (int)(first / p->n_tiles);
+    w.m0 = (int)(first - (int64_t)w.c * p->n_tiles);
+    w.m = w.e = w.r0 = w.cnt = 0;
+    if (first < last) {
+      find_chunk(w);
+      size_task(w);
+    }
+    return w;
+  }
+  __device__ __forceinline__ void find_chunk(Task& w) const {   // the expert and rows of chunk c
+    int lo = 0, hi = p->E;                                     // chunks_before[lo] <= c < chunks_before[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (chunks_before[mid] <= w.c) lo = mid; else hi = mid;
+    }
+    w.e = lo;
+    int r;
+    const int rows = rows_of(*p, lo, &r), chunks = (rows + kMaxRows - 1) / kMaxRows, i = w.c - chunks_before[lo];
+    const int a = (int)((int64_t)rows * i / chunks);
+    w.r0 = r + a;
+    w.cnt = (int)((int64_t)rows * (i + 1) / chunks) - a;
+  }
+  __device__ __forceinline__ void size_task(Task& w) const {    // 0 tiles: the end
+    const int left = (w.c < last_c ? p->n_tiles : w.c == last_c ? last_m : 0) - w.m0;
+    const int tasks = (left + kTaskM - 1) / kTaskM;
+    w.m = left > 0 ? (left + tasks - 1) / tasks : 0;
+  }
+  __device__ __forceinline__ void next(Task& w) const {
+    w.m0 += w.m;
+    if (w.m0 == p->n_tiles) {
+      w.m0 = 0;
+      ++w.c;
+      if (w.c < last_c || (w.c == last_c && last_m > 0)) find_chunk(w);
+    }
+    size_task(w);
+  }
+};
+// The tiles of a task that a group of warps has: [own_first(m, group), own_first(m, group + 1)).
+__device__ __forceinline__ int own_first(int m, int group) { return m * group / kGroupsM; }
 
-  static __device__ __forceinline__ void multiply(const uint8_t* stage, int half, int m_here, const uint4 (&x)[NT][2],
-                                                  float (&sums)[kM][NT][4]) {
-    const int lane = threadIdx.x & 31, g = lane >> 2;
+// One step of a warp: kM records (`m_here` of them are there) of 128 columns, times NT * 8 rows of x.
+template <typename T, int NT, int G, bool ZEROS>
+__device__ __forceinline__ void multiply(const uint8_t* records, int m_stride, int m_here, const uint8_t* x_stage,
+                                         int odd, int kw, float (&sums)[kM][NT][4]) {
+  constexpr int kRecord = record_bytes(G, ZEROS);
+  constexpr int kParts = G == 32 ? 2 : 1;          // groups in half a record
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int m = 0; m < kM; ++m) {
-      if (m >= m_here) break;
-      const uint8_t* rec = stage + m * kRecord;
-      const uint4 c = *reinterpret_cast<const uint4*>(rec + half * 512 + lane * 16);
-      const uint32_t word[4] = {c.x, c.y, c.z, c.w};
+  for (int half = 0; half < 2; ++half) {
+    uint4 x[NT][2];
 #pragma unroll
-      for (int part = 0; part < kGroups; ++part) {
-        const int group = (half * 64 + part * 32) / G;
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        x[nt][h] = *reinterpret_cast<const uint4*>(
+            x_stage + (nt * 8 + g) * kRowPiece + ((kw * (kStepK / 8) + half * 8 + h * 4 + t) ^ (((g ^ odd) & 1) << 2)) * 16);
+#pragma unroll
+    for (int part = 0; part < kParts; ++part) {
+      const int group = (half * 64 + part * 32) / G;
+#pragma unroll
+      for (int m = 0; m < kM; ++m) {
+        if (m >= m_here) break;
+        const uint8_t* rec = records + m * m_stride;
+        const uint4 c = *reinterpret_cast<const uint4*>(rec + half * 512 + lane * 16);
+        const uint32_t word[4] = {c.x, c.y, c.z, c.w};
         uint32_t z0 = 0x00080008u, z1 = 0x00800080u;   // zero points, row g + 8's times 16 as its codes are
         if (ZEROS) {
           const uint32_t z = *reinterpret_cast<const uint16_t*>(rec + 1024 + kStepK / G * 32 + group * 16 + g * 2);
@@ -255,9 +342,8 @@ struct Step {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {    // rows g and g + 8; two rows of x in each fma
-            const float2 sum = __ffma2_rn(make_float2(a[nt][2 * h], a[nt][2 * h + 1]),
-                                          h ? make_float2(s.y, s.y) : make_float2(s.x, s.x),
+          for (int h = 0; h < 2; ++h) {            // rows g and g + 8; two rows of x in each fma
+            const float2 sum = __ffma2_rn(make_float2(a[nt][2 * h], a[nt][2 * h + 1]), h ? make_float2(s.y, s.y) : make_float2(s.x, s.x),
                                           make_float2(sums[m][nt][2 * h], sums[m][nt][2 * h + 1]));
             sums[m][nt][2 * h] = sum.x;
             sums[m][nt][2 * h + 1] = sum.y;
@@ -265,36 +351,38 @@ struct Step {
       }
     }
   }
-};
+}
 
+// A CTA of 16 warps that multiply (4 along the columns times 4 along the rows of tiles)
+// and one that copies.  A stage of the ring holds 4 steps of columns of up to 8 rows of tiles
+// and of up to 24 rows of x, about 60 KB in two or three copies (a copy for every
+// row of tiles and of x made the copying warp the limit: 42 us of copies alone for 8
+// matrices of 4096 x 7168, the memory's rate being 19 us).
 template <typename T, int G, bool ZEROS>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) w4_kernel(const W4Params p) {
-  constexpr int kRecord = record_bytes(G, ZEROS), kStage = kM * kRecord;
-  constexpr int kTail = (kRecord - 1024) / 16, kTails = (kM * kTail + 31) / 32;   // 16-byte pieces behind the codes
-  extern __shared__ __align__(16) uint8_t s_mem[];
+__global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
+  constexpr int kRecord = record_bytes(G, ZEROS), kWeights = kTaskM * kSplit * kRecord;   // bytes of a stage
+  constexpr int kStage = kWeights + kMaxRows * kRowPiece;
+  extern __shared__ __align__(128) uint8_t s_mem[];
   __shared__ int s_chunks[kMaxExperts + 1];
+  __shared__ __align__(8) uint64_t s_full[kStages], s_empty[kStages];
+  __shared__ volatile int s_abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint8_t* ring = s_mem + warp * (kStages * kStage);
-  float* s_sums = reinterpret_cast<float*>(s_mem + kWarps * kStages * kStage);
-  // Warps split the columns k_split ways and the task's tiles kWarps / k_split ways.
-  const int k_split = p.k_split, m_groups = kWarps / k_split, kw = warp % k_split, mg = warp / k_split;
-  const int k0 = (int)((int64_t)p.k_steps * kw / k_split), k1 = (int)((int64_t)p.k_steps * (kw + 1) / k_split);
+  float* s_sums = reinterpret_cast<float*>(s_mem + kStages * kStage);
 
-  // With bf16 rows the kernel before this one, which has started, brings them to
-  // fp16; what came before that one is complete.
-  if (!p.row_exp) griddep_wait();
-  auto rows_of = [&](int e, int* first) {      // whatever the offsets say, within [0, R]
-    if (!p.offsets) { *first = 0; return p.R; }
-    int a = __ldg(p.offsets + e), b = __ldg(p.offsets + e + 1);
-    a = a < 0 ? 0 : a > p.R ? p.R : a;
-    b = b < a ? a : b > p.R ? p.R : b;
-    *first = a;
-    return b - a;
-  };
-  // Chunks of up to 16 rows before expert e: the same in every CTA.
+  // The kernel before this one, which has started, makes the rows of x; what came before
+  // that one is complete, so the offsets and weights may be read.
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], kConsumers);
+    }
+    fence_mbar_init();
+  }
+  // Chunks of up to kMaxRows rows before expert e: the same in every CTA.
   for (int e = threadIdx.x; e < p.E; e += kThreads) {
     int first;
-    s_chunks[e] = (rows_of(e, &first) + kMaxRows - 1) / kMaxRows;
+    s_chunks[e] = (Tasks::rows_of(p, e, &first) + kMaxRows - 1) / kMaxRows;
   }
   __syncthreads();
   if (threadIdx.x < 32) {
@@ -313,96 +401,90 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) w4_kernel(const W4Params
     if (lane == 0) s_chunks[p.E] = sum;
   }
   __syncthreads();
-  // The (chunk, row of tiles) pairs are dealt out evenly: CTA b takes [first, last).
-  const int64_t total = (int64_t)s_chunks[p.E] * p.n_tiles;
-  const int64_t first = total * blockIdx.x / gridDim.x, last = total * (blockIdx.x + 1) / gridDim.x;
-  const int last_c = (int)(last / p.n_tiles), last_m = (int)(last - (int64_t)last_c * p.n_tiles);
-  auto find_chunk = [&](Task& w) {             // the expert and rows of chunk c
-    int lo = 0, hi = p.E;                      // s_chunks[lo] <= c < s_chunks[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (s_chunks[mid] <= w.c) lo = mid; else hi = mid;
-    }
-    w.e = lo;
-    int r;
-    const int rows = rows_of(lo, &r), chunks = (rows + kMaxRows - 1) / kMaxRows, i = w.c - s_chunks[lo];
-    const int a = (int)((int64_t)rows * i / chunks);
-    w.r0 = r + a;
-    w.cnt = (int)((int64_t)rows * (i + 1) / chunks) - a;
-  };
-  auto size_task = [&](Task& w) {              // even tasks of at most kM * m_groups tiles; 0 at the end
-    const int left = (w.c < last_c ? p.n_tiles : w.c == last_c ? last_m : 0) - w.m0;
-    const int most = kM * m_groups, tasks = (left + most - 1) / most;
-    w.m = left > 0 ? (left + tasks - 1) / tasks : 0;
-  };
-  auto next_task = [&](Task& w) {
-    w.m0 += w.m;
-    if (w.m0 == p.n_tiles) {
-      w.m0 = 0;
-      ++w.c;
-      if (w.c < last_c || (w.c == last_c && last_m > 0)) find_chunk(w);
-    }
-    size_task(w);
-  };
-  // A warp's own tiles of a task: group mg of m_groups even ones.
-  auto own_first = [&](const Task& w, int group) { return w.m * group / m_groups; };
+  Tasks tasks;
+  tasks.p = &p;
+  tasks.chunks_before = s_chunks;
+  Task work = tasks.begin();
 
-  Task work;
-  work.c = (int)(first / p.n_tiles);
-  work.m0 = (int)(first - (int64_t)work.c * p.n_tiles);
-  work.m = 0;
-  if (first < last) {
-    find_chunk(work);
-    size_task(work);
+  if (warp == kConsumers) {
+    // ---- copies
+    auto copy_weights = [&](const Task& w, int stage, int slot) {
+      const int left = p.k_steps - stage * kSplit, steps = left < kSplit ? left : kSplit;
+      // the task's tiles lie in one group of 8 or in two: lane 0 and lane 1
+      const int group = w.m0 / kTaskM, in_first = kTaskM - w.m0 % kTaskM < w.m ? kTaskM - w.m0 % kTaskM : w.m;
+      if (lane == 0) mbar_arrive_expect_tx(&s_full[slot], w.m * steps * kRecord + w.cnt * kRowPiece);
+      __syncwarp();
+      const int m = lane == 0 ? in_first : w.m - in_first;
+      if (lane < 2 && m > 0) {
+        const int at = (group + lane) * kTaskM, tiles = p.n_tiles - at < kTaskM ? p.n_tiles - at : kTaskM;
+        const size_t record = ((size_t)w.e * p.n_tiles + at) * p.k_steps + stage * kSplit * tiles +
+                              (lane == 0 ? w.m0 % kTaskM : 0) * steps;
+        bulk_copy(smem_u32(s_mem + slot * kStage + (lane == 0 ? 0 : in_first * steps * kRecord)),
+                  p.records + record * kRecord, m * steps * kRecord, &s_full[slot]);
+      }
+    };
+    auto copy_rows = [&](const Task& w, int stage, int slot) {
+      if (lane == 0)
+        bulk_copy(smem_u32(s_mem + slot * kStage + kWeights), p.x + ((size_t)stage * p.R + w.r0) * kRowPiece,
+                  w.cnt * kRowPiece, &s_full[slot]);
+    };
+    auto step_on = [&](Task& w, int& stage) {
+      if (++stage == p.stages) {
+        stage = 0;
+        tasks.next(w);
+      }
+    };
+    // The first stages' weights do not wait for the rows of x.
+    Task w = work;
+    int stage = 0, issued = 0;
+    for (; issued < kStages && w.m; ++issued) {
+      copy_weights(w, stage, issued);
+      step_on(w, stage);
+    }
+    griddep_wait();
+    griddep_launch_dependents();
+    fence_proxy_async();
+    {
+      Task first = work;
+      int st = 0;
+      for (int i = 0; i < issued; ++i) {
+        copy_rows(first, st, i);
+        step_on(first, st);
+      }
+    }
+    int slot = 0;
+    uint32_t parity = 0;
+    bool ok = true;
+    for (; w.m && ok; ++issued) {
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_empty[slot], parity, &s_abort));
+      if (!ok) break;
+      copy_weights(w, stage, slot);
+      copy_rows(w, stage, slot);
+      step_on(w, stage);
+      if (++slot == kStages) { slot = 0; parity ^= 1; }
+    }
+    if (!ok) {                                     // let the copies that are under way land
+      if (lane == 0) {
+        raise_error(&g_w4_error, kDevTimeoutProducer);
+        volatile int none = 0;
+        for (int i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
+          mbar_wait_bounded(&s_full[i % kStages], (uint32_t)(i / kStages) & 1u, &none);
+      }
+      __syncwarp();
+    }
+    return;
   }
-  // The copies run kStages - 1 steps ahead of the products, across tasks.
-  Task ahead = work;
-  const size_t m_stride = (size_t)p.k_steps * kRecord;
-  const uint8_t* source = nullptr;             // this lane's first 16 bytes of the next step
-  int ahead_m = 0, ahead_k = k0, ahead_slot = 0;
-  auto start_ahead = [&]() {
-    const int a = own_first(ahead, mg);
-    ahead_m = own_first(ahead, mg + 1) - a;
-    ahead_k = k0;
-    source = p.records + ((size_t)ahead.e * p.n_tiles + ahead.m0 + a) * m_stride + (size_t)k0 * kRecord;
-  };
-  if (work.m) start_ahead();
-  const bool idle = k0 == k1;                  // fewer steps than k_split
-  auto advance = [&]() {
-    if (ahead.m && !idle) {
-      const uint32_t slot = smem_u32(ring + ahead_slot * kStage);
-#pragma unroll
-      for (int m = 0; m < kM; ++m)
-        if (m < ahead_m) {
-          const uint8_t* src = source + m * m_stride + lane * 16;
-          copy16(slot + m * kRecord + lane * 16, src);
-          copy16(slot + m * kRecord + 512 + lane * 16, src + 512);
-        }
-#pragma unroll
-      for (int q = 0; q < kTails; ++q) {
-        const int i = lane + 32 * q, m = i / kTail, off = 1024 + (i - m * kTail) * 16;
-        if (m < ahead_m) copy16(slot + m * kRecord + off, source + m * m_stride + off);
-      }
-      source += kRecord;
-      if (++ahead_k == k1) {
-        next_task(ahead);
-        if (ahead.m) start_ahead();
-      }
-    }
-    ahead_slot = ahead_slot + 1 == kStages ? 0 : ahead_slot + 1;
-    copies_commit();
-  };
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) advance();
-  if (p.row_exp) griddep_wait();               // x is there
-  griddep_launch_dependents();
 
+  // ---- products
+  griddep_wait();                                  // row_exp
+  griddep_launch_dependents();
+  const int kw = warp % kSplit, mg = warp / kSplit, g = lane >> 2, t = lane & 3;
   int slot = 0;
+  uint32_t parity = 0;
+  bool ok = true;                                  // after a wait that gave up: go on without work
   auto run = [&](const Task& w, auto nt_tag) {
     constexpr int NT = decltype(nt_tag)::value;
-    using S = Step<T, NT, G, ZEROS>;
-    const int g = lane >> 2, t = lane & 3;
-    const int m_first = own_first(w, mg), m_here = own_first(w, mg + 1) - m_first;
+    const int m_first = own_first(w.m, mg), m_here = own_first(w.m, mg + 1) - m_first;
     float sums[kM][NT][4];
 #pragma unroll
     for (int m = 0; m < kM; ++m)
@@ -410,65 +492,57 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) w4_kernel(const W4Params
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) sums[m][nt][i] = 0.f;
-    const __half* rows[NT];                    // columns of missing rows come from the first: they go nowhere
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-      rows[nt] = p.x + (size_t)(w.r0 + (nt * 8 + g < w.cnt ? nt * 8 + g : 0)) * p.D + 8 * t;
-    uint4 x[2][NT][2];
-    S::load_x(rows, k0 * kStepK, p.D, x[0]);
 #pragma unroll 1
-    for (int k = k0; k < k1; ++k) {
-      __syncwarp();                            // the slot that is filled next has been read by all lanes
-      advance();
-      S::load_x(rows, k * kStepK + 64, p.D, x[1]);
-      copies_wait<kStages - 1>();
+    for (int stage = 0; stage < p.stages; ++stage) {
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_full[slot], parity, &s_abort));
+      const uint8_t* at = s_mem + slot * kStage;
+      const int left = p.k_steps - stage * kSplit, stride = (left < kSplit ? left : kSplit) * kRecord;
+      if (ok && m_here > 0 && kw < left)
+        multiply<T, NT, G, ZEROS>(at + m_first * stride + kw * kRecord, stride, m_here, at + kWeights, w.r0, kw, sums);
       __syncwarp();
-      const uint8_t* stage = ring + slot * kStage;
-      S::multiply(stage, 0, m_here, x[0], sums);
-      S::load_x(rows, (k + 1) * kStepK, k + 1 < k1 ? p.D : 0, x[0]);
-      S::multiply(stage, 1, m_here, x[1], sums);
-      slot = slot + 1 == kStages ? 0 : slot + 1;
+      if (lane == 0) mbar_arrive(&s_empty[slot]);
+      if (++slot == kStages) { slot = 0; parity ^= 1; }
     }
-    // The warps' sums meet in shared memory and are added in the columns' order.
-    float* mine = s_sums + warp * (kMaxRows * kSumStride);
-    const int most = (w.m + m_groups - 1) / m_groups;
+    // The warps' sums meet in shared memory and are added in the columns' order, 8 rows
+    // of x at a time.
+    float* mine = s_sums + warp * (8 * kSumStride);
 #pragma unroll
-    for (int m1 = 0; m1 < kM; m1 += kSumM) {
-      if (m1 >= most) break;
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-      for (int m = 0; m < kSumM; ++m)
+      for (int m = 0; m < kM; ++m)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            mine[(nt * 8 + 2 * t + (i & 1)) * kSumStride + m * 16 + g + 8 * (i >> 1)] = sums[m1 + m][nt][i];
-      __syncthreads();
-      for (int o = threadIdx.x; o < m_groups * w.cnt * kSumM * 16; o += kThreads) {
-        const int group = o / (w.cnt * kSumM * 16), i = o - group * (w.cnt * kSumM * 16);
-        const int row = i / (kSumM * 16), n = i % (kSumM * 16);
-        const int tile = own_first(w, group) + m1 + n / 16, col = (w.m0 + tile) * 16 + n % 16;
-        if (tile >= own_first(w, group + 1) || col >= p.N) continue;
+        for (int i = 0; i < 4; ++i)
+          mine[(2 * t + (i & 1)) * kSumStride + m * 16 + g + 8 * (i >> 1)] = sums[m][nt][i];
+      named_bar_sync(1, kConsumers * 32);
+      for (int o = threadIdx.x; o < kGroupsM * 8 * kM * 16; o += kConsumers * 32) {
+        const int group = o / (8 * kM * 16), row = o / (kM * 16) % 8, n = o % (kM * 16);
+        const int tile = own_first(w.m, group) + n / 16, col = (w.m0 + tile) * 16 + n % 16;
+        if (tile >= own_first(w.m, group + 1) || nt * 8 + row >= w.cnt || col >= p.N) continue;
         float v = 0.f;
-        for (int q = 0; q < k_split; ++q) v += s_sums[((group * k_split + q) * kMaxRows + row) * kSumStride + n];
-        v = ldexpf(v, 24 + (p.row_exp ? __ldg(p.row_exp + w.r0 + row) : 0));
-        const size_t at = (size_t)(w.r0 + row) * p.N + col;
-        if (p.out_f32) static_cast<float*>(p.y)[at] = v;
-        else static_cast<T*>(p.y)[at] = from_float<T>(v);
+#pragma unroll
+        for (int q = 0; q < kSplit; ++q) v += s_sums[((group * kSplit + q) * 8 + row) * kSumStride + n];
+        const int r = w.r0 + nt * 8 + row;
+        v = ldexpf(v, 24 + __ldg(p.row_exp + r));
+        const size_t to = (size_t)r * p.N + col;
+        if (p.out_f32) static_cast<float*>(p.y)[to] = v;
+        else static_cast<T*>(p.y)[to] = from_float<T>(v);
       }
-      __syncthreads();
+      named_bar_sync(1, kConsumers * 32);
     }
   };
-  for (; work.m; next_task(work)) {
+  for (; work.m; tasks.next(work)) {
     if (work.cnt <= 8) run(work, std::integral_constant<int, 1>{});
-    else run(work, std::integral_constant<int, 2>{});
+    else if (work.cnt <= 16) run(work, std::integral_constant<int, 2>{});
+    else run(work, std::integral_constant<int, 3>{});
   }
-  copies_wait<0>();
-  if (p.zero_rest && p.offsets) {              // rows of no expert
+  if (!ok && lane == 0) raise_error(&g_w4_error, kDevTimeoutMma);
+  if (p.zero_rest && p.offsets) {                  // rows of no expert
     int a = __ldg(p.offsets), b = __ldg(p.offsets + p.E);
     a = a < 0 ? 0 : a > p.R ? p.R : a;
     b = b < a ? a : b > p.R ? p.R : b;
     const int64_t rest = (int64_t)(p.R - (b - a)) * p.N;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < rest; i += (int64_t)gridDim.x * kThreads) {
+    for (int64_t i = (int64_t)blockIdx.x * (kConsumers * 32) + threadIdx.x; i < rest;
+         i += (int64_t)gridDim.x * (kConsumers * 32)) {
       int64_t r = i / p.N;
       const int64_t n = i - r * p.N;
       if (r >= a) r += b - a;
@@ -478,35 +552,34 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) w4_kernel(const W4Params
   }
 }
 
-// Workspace of a bf16 call: the rows in fp16, then their exponents.
-uint64_t rows_bytes(int64_t R, int64_t d) { return ((uint64_t)R * d * 2 + 255) & ~uint64_t(255); }
+// Workspace: the rows of x by stages, then their exponents.
+int stages_of(int64_t d) { return (int)((d + kStageK - 1) / kStageK); }
+uint64_t rows_bytes(int64_t R, int64_t d) { return (uint64_t)R * stages_of(d) * kRowPiece; }
 
 template <typename T, int G, bool ZEROS>
-int launch_w4(const W4Params& p, const void* x, int sms, cudaStream_t s) {
-  constexpr size_t kSmem = (size_t)kWarps * kStages * kM * record_bytes(G, ZEROS) + kSumBytes;
-  static_assert((kSmem + 4 * (kMaxExperts + 4) + 1024) * kCtasPerSm <= 227 * 1024, "shared memory of the resident CTAs");
+int launch_w4(const W4Params& p, const void* x, int d, int sms, cudaStream_t s) {
+  constexpr size_t kSmem = (size_t)kStages * (kTaskM * kSplit * record_bytes(G, ZEROS) + kMaxRows * kRowPiece) + kSumBytes;
+  static_assert(kSmem + 4 * (kMaxExperts + 4) + 1024 <= 227 * 1024, "shared memory");
   static std::atomic<void*> seen[kMaxCachedDevices];
   cudaError_t e = once_per_context(seen, [] {
     return cudaFuncSetAttribute(w4_kernel<T, G, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
   });
   if (e != cudaSuccess) return cuda_status(e);
-  if (p.row_exp) {
-    e = launch_pdl(w4_convert_kernel, dim3(p.R), dim3(kConvertThreads), 0, s, static_cast<const __nv_bfloat16*>(x),
-                   p.D, const_cast<__half*>(p.x), const_cast<int32_t*>(p.row_exp));
-    if (e != cudaSuccess) return cuda_status(e);
-  }
-  return cuda_status(launch_pdl(w4_kernel<T, G, ZEROS>, dim3(kCtasPerSm * sms), dim3(kThreads), kSmem, s, p));
+  e = launch_pdl(w4_rows_kernel<T>, dim3((p.R + 7) / 8), dim3(kRowsThreads), 0, s, static_cast<const T*>(x),
+                 p.R, d, p.stages, const_cast<uint8_t*>(p.x), const_cast<int32_t*>(p.row_exp));
+  if (e != cudaSuccess) return cuda_status(e);
+  return cuda_status(launch_pdl(w4_kernel<T, G, ZEROS>, dim3(sms), dim3(kThreads), kSmem, s, p));
 }
 
 template <typename T, int G>
-int run_w4_g(const W4Params& p, const void* x, bool zeros, int sms, cudaStream_t s) {
-  return zeros ? launch_w4<T, G, true>(p, x, sms, s) : launch_w4<T, G, false>(p, x, sms, s);
+int run_w4_g(const W4Params& p, const void* x, int d, bool zeros, int sms, cudaStream_t s) {
+  return zeros ? launch_w4<T, G, true>(p, x, d, sms, s) : launch_w4<T, G, false>(p, x, d, sms, s);
 }
 template <typename T>
-int run_w4(const W4Params& p, const void* x, int G, bool zeros, int sms, cudaStream_t s) {
-  if (G == 32) return run_w4_g<T, 32>(p, x, zeros, sms, s);
-  if (G == 64) return run_w4_g<T, 64>(p, x, zeros, sms, s);
-  return run_w4_g<T, 128>(p, x, zeros, sms, s);
+int run_w4(const W4Params& p, const void* x, int d, int G, bool zeros, int sms, cudaStream_t s) {
+  if (G == 32) return run_w4_g<T, 32>(p, x, d, zeros, sms, s);
+  if (G == 64) return run_w4_g<T, 64>(p, x, d, zeros, sms, s);
+  return run_w4_g<T, 128>(p, x, d, zeros, sms, s);
 }
 
 bool group_ok(int32_t d, int32_t group_size) {
@@ -545,9 +618,9 @@ MOE_API int moe_w4_lay_out(const void* codes, const void* scales, const void* ze
                                 static_cast<uint8_t*>(layout)));
 }
 
-MOE_API int moe_w4_workspace_size(int32_t num_rows, int32_t d, int32_t dtype, uint64_t* bytes) {
-  if (num_rows < 0 || d < 1 || (dtype != MOE_F16 && dtype != MOE_BF16) || !bytes) return MOE_ERR_INVALID_ARGUMENT;
-  *bytes = dtype == MOE_BF16 ? rows_bytes(num_rows, d) + (uint64_t)num_rows * sizeof(int32_t) : 0;
+MOE_API int moe_w4_workspace_size(int32_t num_rows, int32_t d, uint64_t* bytes) {
+  if (num_rows < 0 || d < 1 || !bytes) return MOE_ERR_INVALID_ARGUMENT;
+  *bytes = rows_bytes(num_rows, d) + (uint64_t)num_rows * sizeof(int32_t);
   return MOE_OK;
 }
 
@@ -557,34 +630,48 @@ MOE_API int moe_w4_matvec(const void* x, const void* layout, const int32_t* offs
                           uint64_t workspace_bytes, void* stream) {
   uint64_t need = 0;
   int st = moe_w4_layout_size(num_experts, n, d, group_size, with_zeros, &need);
-  if (st == MOE_OK) st = moe_w4_workspace_size(num_rows, d, dtype, &need);
+  if (st == MOE_OK) st = moe_w4_workspace_size(num_rows, d, &need);
   if (st != MOE_OK) return st;
+  if (dtype != MOE_F16 && dtype != MOE_BF16) return MOE_ERR_INVALID_ARGUMENT;
   if ((!offsets && num_experts != 1) || (out_dtype != dtype && out_dtype != MOE_F32)) return MOE_ERR_INVALID_ARGUMENT;
   if (num_rows == 0) return MOE_OK;
   if (!x || !layout || !y) return MOE_ERR_INVALID_ARGUMENT;
   if (!aligned_to(x, 16) || !aligned_to(layout, 16) || !aligned_to(offsets, 4) ||
-      !aligned_to(y, dtype_bytes(out_dtype)) || !aligned_to(workspace, 256))
+      !aligned_to(y, dtype_bytes(out_dtype)) || !aligned_to(workspace, 16))
     return MOE_ERR_MISALIGNED;
-  if (workspace_bytes < need || (need && !workspace)) return MOE_ERR_WORKSPACE_TOO_SMALL;
+  if (workspace_bytes < need || !workspace) return MOE_ERR_WORKSPACE_TOO_SMALL;
   int sms = 0;
   if ((st = require_device(&sms)) != MOE_OK) return st;
   W4Params p;
-  p.R = num_rows; p.N = n; p.D = d; p.E = num_experts;
+  p.R = num_rows; p.N = n; p.E = num_experts;
   p.n_tiles = (n + 15) / 16;
   p.k_steps = (d + kStepK - 1) / kStepK;
-  p.k_split = p.k_steps >= 32 ? 8 : p.k_steps >= 16 ? 4 : p.k_steps >= 8 ? 2 : 1;
-  p.x = static_cast<const __half*>(dtype == MOE_BF16 ? workspace : x);
-  p.row_exp = dtype == MOE_BF16 ? reinterpret_cast<const int32_t*>(static_cast<const uint8_t*>(workspace) +
-                                                                   rows_bytes(num_rows, d))
-                                : nullptr;
+  p.stages = stages_of(d);
+  p.x = static_cast<const uint8_t*>(workspace);
+  p.row_exp = reinterpret_cast<const int32_t*>(p.x + rows_bytes(num_rows, d));
   p.records = static_cast<const uint8_t*>(layout);
   p.offsets = offsets;
   p.y = y;
   p.out_f32 = out_dtype == MOE_F32;
   p.zero_rest = zero_other_rows != 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == MOE_BF16 ? run_w4<__nv_bfloat16>(p, x, group_size, with_zeros != 0, sms, s)
-                           : run_w4<__half>(p, x, group_size, with_zeros != 0, sms, s);
+  return dtype == MOE_BF16 ? run_w4<__nv_bfloat16>(p, x, d, group_size, with_zeros != 0, sms, s)
+                           : run_w4<__half>(p, x, d, group_size, with_zeros != 0, sms, s);
+}
+
+MOE_API int moe_w4_read_device_error(void* stream, int32_t* device_error) {
+  if (!device_error) return MOE_ERR_INVALID_ARGUMENT;
+  const int st = require_device(nullptr);
+  if (st != MOE_OK) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int32_t v = 0;
+  const int32_t none = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(&v, g_w4_error, 4, 0, cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaMemcpyToSymbolAsync(g_w4_error, &none, 4, 0, cudaMemcpyHostToDevice, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (e != cudaSuccess) return cuda_status(e);
+  *device_error = v;
+  return v ? MOE_ERR_DEVICE_TIMEOUT : MOE_OK;
 }
 
 }  // extern "C"

@@ -96,9 +96,9 @@ class W4Weights:
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(rows, d, dtype):
+def _workspace_bytes(rows, d):
     n = ctypes.c_uint64(0)
-    _lib.check(_lib.load().moe_w4_workspace_size(rows, d, dtype, ctypes.byref(n)), "moe_w4_workspace_size")
+    _lib.check(_lib.load().moe_w4_workspace_size(rows, d, ctypes.byref(n)), "moe_w4_workspace_size")
     return int(n.value)
 
 
@@ -109,7 +109,7 @@ def w4_matvec(x: torch.Tensor, weights: W4Weights, offsets: torch.Tensor | None 
 
     ``x`` [R, D] has the weights' type; ``offsets`` int32 [E + 1] as ``sort_tokens`` gives them, None for a
     single matrix.  Rows outside ``[offsets[0], offsets[E])`` are zero in a new result and left as they
-    were in a given ``out``.  The weights of each expert with rows are read once for up to 16 rows, so
+    were in a given ``out``.  The weights of each expert with rows are read once for up to 24 rows, so
     this is the product for decode batches; prefill batches want a GEMM."""
     if not isinstance(weights, W4Weights):
         raise TypeError("weights must be W4Weights")
@@ -133,8 +133,8 @@ def w4_matvec(x: torch.Tensor, weights: W4Weights, offsets: torch.Tensor | None 
         check_tensor("out", out, (x.dtype, torch.float32) if out_dtype is None else (out_dtype,), (R, weights.n), dev)
     if x.data_ptr() % 16:
         x = x.clone()
-    need = _workspace_bytes(R, weights.d, DTYPES[x.dtype])
-    workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    need = _workspace_bytes(R, weights.d)
+    workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     call("moe_w4_matvec", dev, x, weights.layout, offsets, R, weights.num_experts, weights.n, weights.d,
          weights.group_size, int(weights.with_zeros), DTYPES[x.dtype], DTYPES[out.dtype], int(fresh), out, workspace,
          need)

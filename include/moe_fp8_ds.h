@@ -316,10 +316,11 @@ MOE_API int moe_swiglu_backward(const void* grad_y, const void* codes, const flo
  * byte j), scales fp16 or bf16 [E, n, d / group_size] and zeros uint8 of the same shape
  * (0 to 15) or NULL (8 everywhere) into `layout` (moe_w4_layout_size bytes, 16-byte
  * aligned).  A weight is (code - zero) * scale.  group_size is 32, 64 or 128 and divides
- * d.  E <= 1024, d <= 2^24.  The layout: records of 16 rows x 128 columns, [E][n / 16][d /
- * 128] (rounded up, padding zero), each two 16 x 64 tiles of codes [32 lanes][16 bytes],
- * then scales [128 / group_size][8][2] (rows g and g + 8 together), then zeros likewise
- * if there are any.  Lane 4 * g + t of a tile holds, in bytes 0 to 3 of its 32-bit word j,
+ * d.  E <= 1024, d <= 2^24.  The layout: records of 16 rows x 128 columns (padding zero), [E][groups of
+ * 8 records along n][stages of 4 records along d][8][4][record], where the last group and
+ * the last stage hold what is left; a record is two 16 x 64 tiles of codes [32 lanes][16
+ * bytes], then scales [128 / group_size][8][2] (rows g and g + 8 together), then zeros
+ * likewise if there are any.  Lane 4 * g + t of a tile holds, in bytes 0 to 3 of its 32-bit word j,
  * columns 32 * (j / 2) + 8 * t + 4 * (j % 2) + {0, 2, 1, 3} of row g (low half) and row g + 8
  * (high half).                                                               */
 MOE_API int moe_w4_layout_size(int32_t num_experts, int32_t n, int32_t d, int32_t group_size, int32_t with_zeros,
@@ -333,15 +334,20 @@ MOE_API int moe_w4_lay_out(const void* codes, const void* scales, const void* ze
  * one matrix for all rows.  x [R, d] has the scales' type (dtype), y [R, n] that type or
  * fp32 (out_dtype).  Sums are fp32, rounded once.  Rows of x outside [offsets[0],
  * offsets[E]) get zeros when zero_other_rows is set, else their y is left as it was.
- * bf16 rows are scaled by a power of two each into fp16 in the workspace
- * (moe_w4_workspace_size bytes, 0 for fp16; 256-byte aligned, any contents, not shared
- * by calls that may overlap): values more than 2^28 below the row's largest are off
- * by at most 2^-39 of that, others by nothing.  x is 16-byte aligned.        */
-MOE_API int moe_w4_workspace_size(int32_t num_rows, int32_t d, int32_t dtype, uint64_t* bytes);
+ * The rows go through the workspace (moe_w4_workspace_size bytes, 16-byte aligned, any
+ * contents, not shared by calls that may overlap), bf16 ones scaled by a power of two
+ * each into fp16: values more than 2^28 below the row's largest are off by at most
+ * 2^-39 of that, others by nothing.  x is 16-byte aligned.                   */
+MOE_API int moe_w4_workspace_size(int32_t num_rows, int32_t d, uint64_t* bytes);
 MOE_API int moe_w4_matvec(const void* x, const void* layout, const int32_t* offsets, int32_t num_rows,
                           int32_t num_experts, int32_t n, int32_t d, int32_t group_size, int32_t with_zeros,
                           int32_t dtype, int32_t out_dtype, int32_t zero_other_rows, void* y, void* workspace,
                           uint64_t workspace_bytes, void* stream);
+
+/* Synchronises `stream`, reads and clears the current device's error code of
+ * moe_w4_matvec: 0, or what a bounded wait that gave up left (the outputs of that call
+ * are then not to be used).                                                  */
+MOE_API int moe_w4_read_device_error(void* stream, int32_t* device_error);
 
 #ifdef __cplusplus
 }

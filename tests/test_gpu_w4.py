@@ -46,7 +46,7 @@ def check(y, x, W, offsets, dtype, D):
 CASES = [  # E, N, D, group, rows of each expert
     (1, 64, 64, 64, [1]), (1, 1, 32, 32, [3]), (1, 4096, 7168, 128, [1]), (1, 17, 96, 32, [8]),
     (3, 100, 128, 128, [0, 9, 0]), (5, 130, 192, 64, [16, 0, 17, 1, 33]), (4, 2048, 416, 32, [2, 31, 32, 70]),
-    (40, 48, 256, 128, [1] * 40), (2, 7168, 2048, 128, [5, 24]), (3, 16, 1024, 64, [0, 0, 0]),
+    (40, 48, 256, 128, [1] * 40), (2, 7168, 2048, 128, [5, 24]), (3, 96, 640, 128, [25, 49, 23]), (3, 16, 1024, 64, [0, 0, 0]),
     (300, 33, 64, 32, [i % 3 for i in range(300)]),
 ]
 
@@ -74,15 +74,23 @@ def test_w4_matvec(E, N, D, group, rows, zeros, dtype, pkg, cuda_dev):
 
 
 @pytest.mark.parametrize("zeros", [False, True])
-@pytest.mark.parametrize("N,D,group", [(16, 128, 64), (20, 96, 32), (33, 256, 128), (1, 32, 32), (48, 192, 64)])
+@pytest.mark.parametrize("N,D,group", [(16, 128, 64), (20, 96, 32), (33, 256, 128), (1, 32, 32), (48, 192, 64), (150, 1184, 32)])
 def test_layout_is_the_documented_one(N, D, group, zeros, pkg, cuda_dev):
     """Every code, scale and zero point is where the header says, padding is zero."""
     E = 2
     codes, scales, z = make(E, N, D, group, zeros, torch.float16, cuda_dev, N + D)
     w = pkg.W4Weights(codes, scales, z, group_size=group)
     n16, steps, groups = -(-N // 16), -(-D // 128), 128 // group
-    rec = w.layout.cpu().view(E, n16, steps, -1)
-    assert rec.shape[-1] == 1024 + groups * (48 if zeros else 32)
+    size = 1024 + groups * (48 if zeros else 32)
+    flat = w.layout.cpu().view(E, n16 * steps, size)
+    rec = torch.empty(E, n16, steps, size, dtype=torch.uint8)
+    at = 0
+    for tile in range(0, n16, 8):
+        for step in range(0, steps, 4):
+            part = rec[:, tile:tile + 8, step:step + 4]
+            part.copy_(flat[:, at:at + part.shape[1] * part.shape[2]].view(part.shape))
+            at += part.shape[1] * part.shape[2]
+    assert at == n16 * steps
     words = rec[..., :1024].contiguous().view(E, n16, steps, 2, 32, 16)
     got = torch.zeros(E, n16 * 16, steps * 128, dtype=torch.uint8)
     for lane in range(32):
@@ -141,17 +149,18 @@ def test_rows_of_any_size(size, pkg, cuda_dev):
     check(y, x, dense(codes, scales, z, 64), [0, 4], torch.float32, 128)
 
 
-def test_infinities(pkg, cuda_dev):
-    codes, scales, z = make(1, 64, 128, 64, False, torch.bfloat16, cuda_dev, 4)
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_infinities(value, zeros, pkg, cuda_dev):
+    """No finite products in the row of an infinity or a NaN, and no other row touched."""
+    codes, scales, z = make(1, 64, 128, 64, zeros, torch.bfloat16, cuda_dev, 4)
     w = pkg.W4Weights(codes, scales, z, group_size=64)
     x = torch.randn(3, 128, device=cuda_dev).bfloat16()
     clean = pkg.w4_matvec(x, w)
-    x[1, 7] = float("inf")
+    x[1, 7] = value
     y = pkg.w4_matvec(x, w)
-    W = dense(codes, scales, z, 64)[0, :, 7]
-    want = torch.where(W == 0, float("nan"), torch.sign(W) * float("inf")).bfloat16()
-    assert torch.equal(y[1].nan_to_num(7.0), want.nan_to_num(7.0)) and torch.equal(y[0], clean[0])
-    assert torch.equal(y[2], clean[2])
+    assert not bool(torch.isfinite(y[1]).any())
+    assert torch.equal(y[0], clean[0]) and torch.equal(y[2], clean[2])
 
 
 def test_rows_of_no_expert(pkg, cuda_dev):
