@@ -8,18 +8,22 @@
 // operands (mma.sync m16n8k16, fp32 sums, weights on the M side): the number 0..15 in
 // the low bits of an fp16 is exactly q * 2^-24 (below 2^-14 fp16 is evenly
 // spaced), four bits higher it is 16 * q * 2^-24, so a 32-bit word of eight codes
-// becomes four operand registers by four masks, one shift and four subtractions of
-// the zero point, all exact.  The factors 2^24 and 1/16 go into the scales and the
-// last step; a group's sum is scaled in fp32, and only the output is rounded.
-// (e4m3 operands, where a byte 0..15 is q * 2^-9, need half the masks, but mma.sync
-// with e4m3 is converted to fp16 here: measured four times the instructions.
-// tcgen05 would want the decoded weights in shared memory or TMEM and 128-row tiles; a
-// decode batch has too few rows of x for that to pay.)
+// becomes four operand registers by four masks and one shift.  A group's sum starts at
+// -zero * (sum of x over the group), made once for each row of x, and is scaled in
+// fp32; the factors 2^24 and 1/16 are left to the last step, and only the output is
+// rounded.
+// What else was built and measured (us; 8 matrices of 4096 x 7168 times a row each /
+// 32 of them times 16 rows): zero points subtracted from the operands, 16 more
+// instructions for each 16 x 64 codes, 40 / 208; e4m3 operands, where a byte 0..15 is
+// q * 2^-9, 55 / 428 (mma.sync with e4m3 is converted to fp16 here, four times the
+// instructions); tcgen05.mma with the decoded weights in tensor memory, 112 / 410 (8
+// products of N = 16 and their hand-overs took 2000 clocks for 128 x 128 codes that
+// arrive in 360).
 //
-// bf16 rows of x are brought to fp16 by a power of two for each row that puts its
-// largest magnitude into [2^14, 2^15): exact for values down to 2^-28 of the largest,
-// below that off by at most 2^-39 of it.  (Next to an infinity or a NaN the finite
-// values vanish, as they do in the sum.)
+// Rows of x are brought to fp16 by a power of two for each row that puts its largest
+// magnitude into [2^14, 2^15): exact for bf16 values down to 2^-28 of the largest,
+// below that off by at most 2^-39 of it; fp16 rows stay as they are.  A row with an
+// infinity or a NaN has no finite products.
 //
 // Layout (made once, by moe_w4_lay_out): records of 16 rows x 128 columns, in the
 // order in which a CTA streams them, so that what it takes at a time is one or two
@@ -41,18 +45,25 @@ namespace {
 
 constexpr int kStepK = 128;               // columns of a record
 constexpr int kSplit = 4;                 // warps along the columns: a stage holds 4 steps
-constexpr int kGroupsM = 4;               // groups of warps along the rows of tiles
-constexpr int kM = 2;                     // rows of tiles (of records) of a warp
+constexpr int kGroupsM = 2;               // groups of warps along the rows of tiles
+constexpr int kM = 4;                     // rows of tiles (of records) of a warp
 constexpr int kTaskM = kM * kGroupsM;     // of a task
-constexpr int kConsumers = kSplit * kGroupsM;       // warps that multiply; one more copies
-constexpr int kThreads = (kConsumers + 1) * 32;
-constexpr int kStages = 3;
+constexpr int kConsumers = kSplit * kGroupsM;       // warps that multiply
+constexpr int kSumsEach = 4 * kM / kSplit;          // sums a thread adds up for 8 rows of x
+constexpr int kGroupSums = 8 * kM * 16;             // of a group's tiles and 8 rows of x
+constexpr int kThreads = (kConsumers + 4) * 32;     // a warpgroup beside them: one of its warps copies
+// Registers a thread: 168 at launch (384 threads share 64,512), then few for that
+// warpgroup and the rest for the two that multiply: 128 * 40 + 256 * 232 = 64,512.
+constexpr int kFewRegisters = 40, kManyRegisters = 232;
+constexpr int kMaxStages = 16;            // of the ring, as many as fit
+constexpr int kEarly = 4;                 // stages whose weights are copied before the rows of x are there
 constexpr int kMaxRows = 24;              // rows of x in a task
 constexpr int kMaxExperts = 1024;
 constexpr int kStageK = kSplit * kStepK;  // columns of a stage
-constexpr int kRowPiece = kStageK * 2;    // bytes of a row of x in a stage
+constexpr int kRowPiece = kStageK * 2 + 64;   // bytes of a row of x in a stage: 512 fp16, then 16 sums of x
 constexpr int kSumStride = kM * 16 + 4;   // of the sums in shared memory: a warp's stores hit 32 banks
 constexpr size_t kSumBytes = sizeof(float) * kConsumers * 8 * kSumStride;
+constexpr size_t kSmem = 225 * 1024 - 8 * (kMaxExperts + 4);   // dynamic: the ring, then the sums
 
 // Bytes of a record with groups of G columns.
 __host__ __device__ constexpr int record_bytes(int G, bool zeros) { return 1024 + kStepK / G * (zeros ? 48 : 32); }
@@ -133,75 +144,86 @@ w4_lay_out_kernel(const uint8_t* __restrict__ codes, const uint16_t* __restrict_
   *reinterpret_cast<uint4*>(out + at * 16) = o.v;
 }
 
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                        uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {   // subnormal numbers included
-  uint32_t d;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
+// d = a * b + c; d may be c.
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1, float c0, float c1, float c2, float c3) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
 // --------------------------------------------------------------------------
-// Rows of x for the product: a CTA takes 8 rows, finds the largest magnitude of each
-// (bf16) and writes them in fp16 by stages of 512 columns, zeros behind D; 16-byte pieces 4
-// apart change places in odd rows, so that a warp's reads of 8 rows hit 32 banks.
-// Reads and writes R * D * 2 bytes, out of and into L2: latency.
+// Rows of x for the product: a CTA takes a row, finds its largest magnitude (bf16) and
+// writes it in fp16 by stages of 512 columns, zeros behind D, each followed by
+// -2^-24 * (sum of x) over its groups (at most 128 columns).  Reads and writes R * D * 2
+// bytes, out of and into L2: latency, so the row is read once, all of it at a time up
+// to 8192 columns.
 // --------------------------------------------------------------------------
-constexpr int kRowsThreads = 512;
+constexpr int kRowsThreads = 512, kRowsHeld = 2;   // threads; 8-column pieces each keeps in registers
 
-template <typename T>
+template <typename T, int G>
 __global__ void __launch_bounds__(kRowsThreads)
 w4_rows_kernel(const T* __restrict__ x, int R, int D, int stages, uint8_t* __restrict__ out,
                int32_t* __restrict__ row_exp) {
-  constexpr int kWarps = kRowsThreads / 32;
   constexpr bool kScaled = !std::is_same<T, __half>::value;
-  __shared__ float s_max[kWarps];
+  __shared__ float s_max[kRowsThreads / 32];
   griddep_wait();
   griddep_launch_dependents();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // warps w and w + 8: the two halves of row w
-  const int row = blockIdx.x * 8 + (warp & 7);
+  const int row = blockIdx.x, width = stages * kStageK;
+  const T* src = x + (size_t)row * D;
+  Pack<T, 8> held[kRowsHeld];
+#pragma unroll
+  for (int i = 0; i < kRowsHeld; ++i) {
+    const int col = (i * kRowsThreads + (int)threadIdx.x) * 8;            // D is a multiple of 32
+    held[i] = col < D ? load_cached<T, 8>(src + col) : zero_pack<T, 8>();
+  }
   int exp = 0;
   if constexpr (kScaled) {
     float amax = 0.f;
-    if (row < R)
-#pragma unroll 4
-      for (int i = (warp >> 3) * 256 + lane * 8; i < D; i += 512) {   // D is a multiple of 32
-        const Pack<T, 8> v = load_cached<T, 8>(x + (size_t)row * D + i);
+    auto look = [&](const Pack<T, 8>& v) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float a = fabsf(to_float(v.v[j]));
-          amax = a < INFINITY ? fmaxf(amax, a) : INFINITY;
-        }
+      for (int j = 0; j < 8; ++j) {
+        const float a = fabsf(to_float(v.v[j]));
+        amax = a < INFINITY ? fmaxf(amax, a) : INFINITY;
       }
+    };
+#pragma unroll
+    for (int i = 0; i < kRowsHeld; ++i) look(held[i]);
+    for (int col = (kRowsHeld * kRowsThreads + (int)threadIdx.x) * 8; col < D; col += kRowsThreads * 8)
+      look(load_cached<T, 8>(src + col));
 #pragma unroll
     for (int off = 16; off; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-    if (lane == 0) s_max[warp] = amax;
+    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = amax;
     __syncthreads();
-    amax = fmaxf(s_max[warp & 7], s_max[(warp & 7) + 8]);
+#pragma unroll
+    for (int i = 0; i < kRowsThreads / 32; ++i) amax = fmaxf(amax, s_max[i]);
     // amax * 2^-exp in [2^14, 2^15), as far as 2^-exp is a normal number
     exp = (int)((__float_as_uint(amax) >> 23) & 0xff) - 127 - 14;
     exp = exp < -120 ? -120 : exp;
   }
-  if (row >= R) return;
   const float down = __uint_as_float((uint32_t)(127 - exp) << 23);
-#pragma unroll 4
-  for (int i = (warp >> 3) * 256 + lane * 8; i < stages * kStageK; i += 512) {
-    Pack<__half, 8> o = zero_pack<__half, 8>();
-    if (i < D) {
-      const Pack<T, 8> v = load_cached<T, 8>(x + (size_t)row * D + i);
+  auto put = [&](int col, const Pack<T, 8>& v) {   // by all threads of a group's columns together
+    Pack<__half, 8> o;
+    float sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        o.v[j] = kScaled ? __float2half_rn(to_float(v.v[j]) * down) : from_float<__half>(to_float(v.v[j]));
+    for (int j = 0; j < 8; ++j) {
+      o.v[j] = __float2half_rn(kScaled ? to_float(v.v[j]) * down : to_float(v.v[j]));
+      sum += to_float(o.v[j]);
     }
-    const int stage = i / kStageK, piece = (i % kStageK / 8) ^ ((row & 1) << 2);
-    store_wide<__half, 8>(reinterpret_cast<__half*>(out + ((size_t)stage * R + row) * kRowPiece) + piece * 8, o);
+#pragma unroll
+    for (int off = 1; off < G / 8; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    uint8_t* piece = out + ((size_t)(col / kStageK) * R + row) * kRowPiece;
+    if (col >= width) return;
+    store_wide<__half, 8>(reinterpret_cast<__half*>(piece) + col % kStageK, o);
+    if (col % G == 0) reinterpret_cast<float*>(piece + kStageK * 2)[col % kStageK / G] = -0x1p-24f * sum;
+  };
+#pragma unroll
+  for (int i = 0; i < kRowsHeld; ++i) put((i * kRowsThreads + (int)threadIdx.x) * 8, held[i]);
+  for (int base = kRowsHeld * kRowsThreads * 8; base < width; base += kRowsThreads * 8) {   // whole CTAs
+    const int col = base + (int)threadIdx.x * 8;
+    put(col, col < D ? load_cached<T, 8>(src + col) : zero_pack<T, 8>());
   }
-  if (warp < 8 && lane == 0) row_exp[row] = exp;
+  if (threadIdx.x == 0) row_exp[row] = exp;
 }
 
 // --------------------------------------------------------------------------
@@ -228,13 +250,16 @@ struct Task {
   int c, e, m0, m, r0, cnt;
 };
 
-// The tasks of a CTA.  The (chunk, row of tiles) pairs are dealt out evenly: CTA b takes the
-// pairs [total * b / CTAs, total * (b + 1) / CTAs), in even tasks of at most kTaskM tiles.
+// The tasks of a CTA.  The (chunk, row of tiles) pairs are dealt out in runs of equal cost, and a
+// CTA's run is split into even tasks of at most kTaskM tiles.
 struct Tasks {
   const W4Params* p;
   const int* chunks_before;   // [E + 1]
-  int last_c, last_m;
+  const int* cost_before;     // [E + 1]: of a row of tiles of all chunks before expert e
+  int last_c, last_m, tiles;
 
+  // No task has more tiles than this.
+  __device__ __forceinline__ int most() const { return tiles < kTaskM ? tiles : kTaskM; }
   // Rows of expert e, whatever the offsets say within [0, R].
   static __device__ __forceinline__ int rows_of(const W4Params& p, int e, int* first) {
     if (!p.offsets) { *first = 0; return p.R; }
@@ -244,16 +269,30 @@ struct Tasks {
     *first = a;
     return b - a;
   }
+  // The pair (chunk, row of tiles), as chunk * n_tiles + tile, at which CTA b starts.
+  __device__ __forceinline__ int start_of(int b) const {
+    const int64_t at = (int64_t)cost_before[p->E] * p->n_tiles * b / (int)gridDim.x;
+    int lo = 0, hi = p->E;                                     // cost_before[lo] * n_tiles <= at
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if ((int64_t)cost_before[mid] * p->n_tiles <= at) lo = mid; else hi = mid;
+    }
+    const int chunks = chunks_before[lo + 1] - chunks_before[lo];
+    if (chunks <= 0) return chunks_before[p->E] * p->n_tiles;  // b is the number of CTAs
+    const int cost = (cost_before[lo + 1] - cost_before[lo]) / chunks;
+    const int tile = (int)((at - (int64_t)cost_before[lo] * p->n_tiles) / cost), most = chunks * p->n_tiles;
+    return chunks_before[lo] * p->n_tiles + (tile < most ? tile : most);
+  }
   __device__ __forceinline__ Task begin() {
-    const int64_t total = (int64_t)chunks_before[p->E] * p->n_tiles;
-    const int64_t first = total * blockIdx.x / gridDim.x, last = total * (blockIdx.x + 1) / gridDim.x;
-    last_c = (int)(last / p->n_tiles);
-    last_m = (int)(last - (int64_t)last_c * p->n_tiles);
+    const int first = start_of(blockIdx.x), last = start_of(blockIdx.x + 1);
+    tiles = last - first;
+    last_c = last / p->n_tiles;
+    last_m = last - last_c * p->n_tiles;
     Task w;
-    w.c = (int)(first / p->n_tiles);
-    w.m0 = (int)(first - (int64_t)w.c * p->n_tiles);
+    w.c = first / p->n_tiles;
+    w.m0 = first - w.c * p->n_tiles;
     w.m = w.e = w.r0 = w.cnt = 0;
-    if (first < last) {
+    if (tiles > 0) {
       find_chunk(w);
       size_task(w);
     }
@@ -268,9 +307,9 @@ struct Tasks {
     w.e = lo;
     int r;
     const int rows = rows_of(*p, lo, &r), chunks = (rows + kMaxRows - 1) / kMaxRows, i = w.c - chunks_before[lo];
-    const int a = (int)((int64_t)rows * i / chunks);
-    w.r0 = r + a;
-    w.cnt = (int)((int64_t)rows * (i + 1) / chunks) - a;
+    const int each = rows / chunks, more = rows - each * chunks;   // even chunks
+    w.r0 = r + each * i + (i < more ? i : more);
+    w.cnt = each + (i < more ? 1 : 0);
   }
   __device__ __forceinline__ void size_task(Task& w) const {    // 0 tiles: the end
     const int left = (w.c < last_c ? p->n_tiles : w.c == last_c ? last_m : 0) - w.m0;
@@ -287,159 +326,221 @@ struct Tasks {
     size_task(w);
   }
 };
+// What a tile costs with this many rows of x, in sixths of the cost with 8: measured with all of 32
+// experts of 4096 x 7168 at 8, 16 and 24 rows (groups of 128: 92, 122, 162 us; of 32: 71, 115, 160).
+template <int G>
+__device__ __forceinline__ int chunk_cost(int rows) {
+  return rows <= 8 ? 6 : rows <= 16 ? (G == 32 ? 9 : 8) : (G == 32 ? 13 : 11);
+}
 // The tiles of a task that a group of warps has: [own_first(m, group), own_first(m, group + 1)).
 __device__ __forceinline__ int own_first(int m, int group) { return m * group / kGroupsM; }
 
-// One step of a warp: kM records (`m_here` of them are there) of 128 columns, times NT * 8 rows of x.
-template <typename T, int NT, int G, bool ZEROS>
-__device__ __forceinline__ void multiply(const uint8_t* records, int m_stride, int m_here, const uint8_t* x_stage,
-                                         int odd, int kw, float (&sums)[kM][NT][4]) {
-  constexpr int kRecord = record_bytes(G, ZEROS);
-  constexpr int kParts = G == 32 ? 2 : 1;          // groups in half a record
+// mbar_wait_bounded, with the clock left alone until a thousand polls have failed: reading it takes
+// longer than most waits here.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+#pragma unroll 1
+  for (int i = 0; i < 1024; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait_bounded(bar, parity, abort_flag);
+}
+
+// One step of a warp: M records of 128 columns, `m_stride` bytes apart, times NT * 8 rows of x.  The
+// records are worked on side by side, so that M * NT chains of products are under way.
+template <typename T, int NT, int M, int G, bool ZEROS>
+__device__ __forceinline__ void multiply(const uint8_t* records, int m_stride, const uint8_t* x_stage, int kw,
+                                         float (&sums)[kM][NT][4]) {
+  constexpr int kParts = kStepK / G, kWords = 8 / kParts;   // groups of the step, words of a lane in each
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  float x_sum[NT][2][kParts];                      // -2^-24 * sums of x, rows 2t and 2t + 1
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    uint4 x[NT][2];
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int i = 0; i < 2; ++i) {
+      const Pack<float, kParts> v = *reinterpret_cast<const Pack<float, kParts>*>(
+          x_stage + (nt * 8 + 2 * t + i) * kRowPiece + kStageK * 2 + kw * kParts * 4);
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        x[nt][h] = *reinterpret_cast<const uint4*>(
-            x_stage + (nt * 8 + g) * kRowPiece + ((kw * (kStepK / 8) + half * 8 + h * 4 + t) ^ (((g ^ odd) & 1) << 2)) * 16);
+      for (int part = 0; part < kParts; ++part) x_sum[nt][i][part] = v.v[part];
+    }
+  float a[M][NT][4];
+  uint4 x[NT][2], codes[M];
 #pragma unroll
-    for (int part = 0; part < kParts; ++part) {
-      const int group = (half * 64 + part * 32) / G;
+  for (int j = 0; j < 8; ++j) {                    // 16 columns each
+    const int part = j / kWords;
+    if (j % 4 == 0) {                              // half a record
 #pragma unroll
-      for (int m = 0; m < kM; ++m) {
-        if (m >= m_here) break;
-        const uint8_t* rec = records + m * m_stride;
-        const uint4 c = *reinterpret_cast<const uint4*>(rec + half * 512 + lane * 16);
-        const uint32_t word[4] = {c.x, c.y, c.z, c.w};
-        uint32_t z0 = 0x00080008u, z1 = 0x00800080u;   // zero points, row g + 8's times 16 as its codes are
-        if (ZEROS) {
-          const uint32_t z = *reinterpret_cast<const uint16_t*>(rec + 1024 + kStepK / G * 32 + group * 16 + g * 2);
-          z0 = (z & 0xff) * 0x00010001u;
-          z1 = (z >> 8) * 0x00100010u;
-        }
-        float a[NT][4];
+      for (int m = 0; m < M; ++m)
+        codes[m] = *reinterpret_cast<const uint4*>(records + m * m_stride + j / 4 * 512 + lane * 16);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) a[nt][i] = 0.f;
+        for (int h = 0; h < 2; ++h)
+          x[nt][h] = *reinterpret_cast<const uint4*>(x_stage + (nt * 8 + g) * kRowPiece +
+                                                     (kw * kStepK + j / 4 * 64 + h * 32 + t * 8) * 2);
+    }
+    const bool first = j % kWords == 0;
 #pragma unroll
-        for (int j = 2 * part; j < (G == 32 ? 2 * part + 2 : 4); ++j) {
-          const uint32_t w = word[j], w8 = w >> 8;
-          const uint32_t a0 = sub_f16x2(w & 0x000f000fu, z0), a1 = sub_f16x2(w & 0x00f000f0u, z1);
-          const uint32_t a2 = sub_f16x2(w8 & 0x000f000fu, z0), a3 = sub_f16x2(w8 & 0x00f000f0u, z1);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const uint4 v = x[nt][j >> 1];
-            mma_f16(a[nt], a0, a1, a2, a3, (j & 1) ? v.z : v.x, (j & 1) ? v.w : v.y);
-          }
-        }
-        float2 s = pair_of<T>(*reinterpret_cast<const uint32_t*>(rec + 1024 + group * 32 + g * 4));
-        s.y *= 0.0625f;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {            // rows g and g + 8; two rows of x in each fma
-            const float2 sum = __ffma2_rn(make_float2(a[nt][2 * h], a[nt][2 * h + 1]), h ? make_float2(s.y, s.y) : make_float2(s.x, s.x),
-                                          make_float2(sums[m][nt][2 * h], sums[m][nt][2 * h + 1]));
-            sums[m][nt][2 * h] = sum.x;
-            sums[m][nt][2 * h + 1] = sum.y;
-          }
+    for (int m = 0; m < M; ++m) {
+      const uint32_t w = j % 4 == 0 ? codes[m].x : j % 4 == 1 ? codes[m].y : j % 4 == 2 ? codes[m].z : codes[m].w;
+      const uint32_t w8 = w >> 8;
+      const uint32_t a0 = w & 0x000f000fu, a1 = w & 0x00f000f0u, a2 = w8 & 0x000f000fu, a3 = w8 & 0x00f000f0u;
+      float z0 = 8.f, z1 = 128.f;                  // zero points, row g + 8's times 16 as its codes are
+      if (ZEROS && first) {
+        const uint32_t v =
+            *reinterpret_cast<const uint16_t*>(records + m * m_stride + 1024 + kParts * 32 + part * 16 + g * 2);
+        z0 = __uint_as_float(0x4b000000u | (v & 0xff)) - 8388608.f;
+        z1 = 16.f * (__uint_as_float(0x4b000000u | v >> 8) - 8388608.f);
       }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const uint4 v = x[nt][j % 4 >> 1];
+        const uint32_t b0 = (j & 1) ? v.z : v.x, b1 = (j & 1) ? v.w : v.y;
+        if (first)
+          mma_f16(a[m][nt], a0, a1, a2, a3, b0, b1, z0 * x_sum[nt][0][part], z0 * x_sum[nt][1][part],
+                  z1 * x_sum[nt][0][part], z1 * x_sum[nt][1][part]);
+        else
+          mma_f16(a[m][nt], a0, a1, a2, a3, b0, b1, a[m][nt][0], a[m][nt][1], a[m][nt][2], a[m][nt][3]);
+      }
+    }
+    if (j % kWords != kWords - 1) continue;
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const float2 s = pair_of<T>(*reinterpret_cast<const uint32_t*>(records + m * m_stride + 1024 + part * 32 + g * 4));
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {              // rows g and g + 8; two rows of x in each fma
+          const float2 sum = __ffma2_rn(make_float2(a[m][nt][2 * h], a[m][nt][2 * h + 1]),
+                                        h ? make_float2(s.y, s.y) : make_float2(s.x, s.x),
+                                        make_float2(sums[m][nt][2 * h], sums[m][nt][2 * h + 1]));
+          sums[m][nt][2 * h] = sum.x;
+          sums[m][nt][2 * h + 1] = sum.y;
+        }
     }
   }
 }
 
-// A CTA of 16 warps that multiply (4 along the columns times 4 along the rows of tiles)
+// A CTA of 8 warps that multiply (4 along the columns times 2 along the rows of tiles)
 // and one that copies.  A stage of the ring holds 4 steps of columns of up to 8 rows of tiles
 // and of up to 24 rows of x, about 60 KB in two or three copies (a copy for every
 // row of tiles and of x made the copying warp the limit: 42 us of copies alone for 8
 // matrices of 4096 x 7168, the memory's rate being 19 us).
 template <typename T, int G, bool ZEROS>
 __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
-  constexpr int kRecord = record_bytes(G, ZEROS), kWeights = kTaskM * kSplit * kRecord;   // bytes of a stage
-  constexpr int kStage = kWeights + kMaxRows * kRowPiece;
+  constexpr int kRecord = record_bytes(G, ZEROS);
   extern __shared__ __align__(128) uint8_t s_mem[];
-  __shared__ int s_chunks[kMaxExperts + 1];
-  __shared__ __align__(8) uint64_t s_full[kStages], s_empty[kStages];
+  __shared__ int s_chunks[kMaxExperts + 1], s_cost[kMaxExperts + 1];
+  __shared__ __align__(8) uint64_t s_full[kMaxStages], s_empty[kMaxStages];
   __shared__ volatile int s_abort;
+  __shared__ int s_most_rows, s_exp[kMaxRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float* s_sums = reinterpret_cast<float*>(s_mem + kStages * kStage);
+  float* s_sums = reinterpret_cast<float*>(s_mem + (kSmem - kSumBytes));
 
   // The kernel before this one, which has started, makes the rows of x; what came before
   // that one is complete, so the offsets and weights may be read.
   if (threadIdx.x == 0) {
     s_abort = 0;
-    for (int i = 0; i < kStages; ++i) {
+    s_most_rows = 0;
+    for (int i = 0; i < kMaxStages; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&s_empty[i], kConsumers);
     }
     fence_mbar_init();
   }
+  __syncthreads();
   // Chunks of up to kMaxRows rows before expert e: the same in every CTA.
   for (int e = threadIdx.x; e < p.E; e += kThreads) {
     int first;
-    s_chunks[e] = (Tasks::rows_of(p, e, &first) + kMaxRows - 1) / kMaxRows;
+    const int rows = Tasks::rows_of(p, e, &first), chunks = (rows + kMaxRows - 1) / kMaxRows;
+    s_chunks[e] = chunks;
+    if (chunks) atomicMax(&s_most_rows, (rows + chunks - 1) / chunks);
+    s_cost[e] = chunks ? chunks * chunk_cost<G>((rows + chunks - 1) / chunks) : 0;
   }
   __syncthreads();
   if (threadIdx.x < 32) {
-    int sum = 0;
+    int sum = 0, cost_sum = 0;
     for (int e0 = 0; e0 < p.E; e0 += 32) {
-      const int e = e0 + lane, v = e < p.E ? s_chunks[e] : 0;
-      int incl = v;
+      const int e = e0 + lane, v = e < p.E ? s_chunks[e] : 0, cost = e < p.E ? s_cost[e] : 0;
+      int incl = v, cost_incl = cost;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, incl, off);
-        if (lane >= off) incl += o;
+        const int o = __shfl_up_sync(0xffffffffu, incl, off), oc = __shfl_up_sync(0xffffffffu, cost_incl, off);
+        if (lane >= off) {
+          incl += o;
+          cost_incl += oc;
+        }
       }
-      if (e < p.E) s_chunks[e] = sum + incl - v;
+      if (e < p.E) {
+        s_chunks[e] = sum + incl - v;
+        s_cost[e] = cost_sum + cost_incl - cost;
+      }
       sum += __shfl_sync(0xffffffffu, incl, 31);
+      cost_sum += __shfl_sync(0xffffffffu, cost_incl, 31);
     }
-    if (lane == 0) s_chunks[p.E] = sum;
+    if (lane == 0) {
+      s_chunks[p.E] = sum;
+      s_cost[p.E] = cost_sum;
+    }
   }
   __syncthreads();
   Tasks tasks;
   tasks.p = &p;
   tasks.chunks_before = s_chunks;
+  tasks.cost_before = s_cost;
   Task work = tasks.begin();
+  // Stages of the ring are as large as this CTA's tasks can need, and as many as fit: where a
+  // CTA has one or two rows of tiles, all of their columns can be on their way at once.
+  const int weights_bytes = tasks.most() * kSplit * kRecord, stage_bytes = weights_bytes + s_most_rows * kRowPiece;
+  const int fit = (int)(kSmem - kSumBytes) / (stage_bytes > 0 ? stage_bytes : 1);
+  const int stages = fit < kMaxStages ? fit : kMaxStages;
 
-  if (warp == kConsumers) {
+  if (warp >= kConsumers) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
+    if (warp > kConsumers) return;
     // ---- copies
-    auto copy_weights = [&](const Task& w, int stage, int slot) {
-      const int left = p.k_steps - stage * kSplit, steps = left < kSplit ? left : kSplit;
-      // the task's tiles lie in one group of 8 or in two: lane 0 and lane 1
-      const int group = w.m0 / kTaskM, in_first = kTaskM - w.m0 % kTaskM < w.m ? kTaskM - w.m0 % kTaskM : w.m;
-      if (lane == 0) mbar_arrive_expect_tx(&s_full[slot], w.m * steps * kRecord + w.cnt * kRowPiece);
+    // Lane 0 and, where a task's tiles lie in two groups of 8, lane 1 copy the weights.
+    struct Source {
+      const uint8_t* at;      // this lane's records of the stage
+      int m, step, tiles, skip, dst;
+    };
+    auto source_of = [&](const Task& w) {
+      Source src;
+      const int in_first = kTaskM - w.m0 % kTaskM < w.m ? kTaskM - w.m0 % kTaskM : w.m;
+      const int at = (w.m0 / kTaskM + (lane & 1)) * kTaskM;
+      src.m = lane == 0 ? in_first : lane == 1 ? w.m - in_first : 0;
+      src.tiles = p.n_tiles - at < kTaskM ? p.n_tiles - at : kTaskM;
+      src.at = p.records + ((size_t)w.e * p.n_tiles + at) * p.k_steps * kRecord;
+      src.step = src.tiles * kSplit * kRecord;
+      src.skip = lane == 0 ? w.m0 % kTaskM : 0;      // tiles of the group before the task's
+      src.dst = lane == 0 ? 0 : in_first;            // tiles of the task before this lane's
+      return src;
+    };
+    auto copy_weights = [&](const Task& w, Source& src, int stage, int slot) {
+      const int left = p.k_steps - stage * kSplit, bytes = (left < kSplit ? left : kSplit) * kRecord;
+      if (lane == 0) mbar_arrive_expect_tx(&s_full[slot], w.m * bytes + w.cnt * kRowPiece);
       __syncwarp();
-      const int m = lane == 0 ? in_first : w.m - in_first;
-      if (lane < 2 && m > 0) {
-        const int at = (group + lane) * kTaskM, tiles = p.n_tiles - at < kTaskM ? p.n_tiles - at : kTaskM;
-        const size_t record = ((size_t)w.e * p.n_tiles + at) * p.k_steps + stage * kSplit * tiles +
-                              (lane == 0 ? w.m0 % kTaskM : 0) * steps;
-        bulk_copy(smem_u32(s_mem + slot * kStage + (lane == 0 ? 0 : in_first * steps * kRecord)),
-                  p.records + record * kRecord, m * steps * kRecord, &s_full[slot]);
-      }
+      if (src.m > 0)
+        bulk_copy(smem_u32(s_mem + slot * stage_bytes + src.dst * bytes), src.at + src.skip * bytes, src.m * bytes,
+                  &s_full[slot]);
+      src.at += src.step;
     };
     auto copy_rows = [&](const Task& w, int stage, int slot) {
-      if (lane == 0)
-        bulk_copy(smem_u32(s_mem + slot * kStage + kWeights), p.x + ((size_t)stage * p.R + w.r0) * kRowPiece,
+      if (lane == 2)
+        bulk_copy(smem_u32(s_mem + slot * stage_bytes + weights_bytes), p.x + ((size_t)stage * p.R + w.r0) * kRowPiece,
                   w.cnt * kRowPiece, &s_full[slot]);
     };
     auto step_on = [&](Task& w, int& stage) {
-      if (++stage == p.stages) {
-        stage = 0;
-        tasks.next(w);
-      }
+      if (++stage < p.stages) return false;
+      stage = 0;
+      tasks.next(w);
+      return true;
     };
-    // The first stages' weights do not wait for the rows of x.
+    // The weights of the first stages do not wait for the rows of x.
     Task w = work;
+    Source src = source_of(w);
     int stage = 0, issued = 0;
-    for (; issued < kStages && w.m; ++issued) {
-      copy_weights(w, stage, issued);
-      step_on(w, stage);
+    for (; issued < kEarly && issued < stages && w.m; ++issued) {
+      copy_weights(w, src, stage, issued);
+      if (step_on(w, stage)) src = source_of(w);
     }
     griddep_wait();
     griddep_launch_dependents();
@@ -452,23 +553,23 @@ __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
         step_on(first, st);
       }
     }
-    int slot = 0;
-    uint32_t parity = 0;
+    int slot = issued == stages ? 0 : issued;
+    uint32_t parity = issued == stages ? 0 : 1;    // a fresh slot counts as freed
     bool ok = true;
-    for (; w.m && ok; ++issued) {
-      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_empty[slot], parity, &s_abort));
+    for (; w.m; ++issued) {
+      ok = __all_sync(0xffffffffu, wait_for(&s_empty[slot], parity, &s_abort));
       if (!ok) break;
-      copy_weights(w, stage, slot);
+      copy_weights(w, src, stage, slot);
       copy_rows(w, stage, slot);
-      step_on(w, stage);
-      if (++slot == kStages) { slot = 0; parity ^= 1; }
+      if (step_on(w, stage)) src = source_of(w);
+      if (++slot == stages) { slot = 0; parity ^= 1; }
     }
     if (!ok) {                                     // let the copies that are under way land
       if (lane == 0) {
         raise_error(&g_w4_error, kDevTimeoutProducer);
         volatile int none = 0;
-        for (int i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
-          mbar_wait_bounded(&s_full[i % kStages], (uint32_t)(i / kStages) & 1u, &none);
+        for (int i = issued > stages ? issued - stages : 0; i < issued; ++i)
+          wait_for(&s_full[i % stages], (uint32_t)(i / stages) & 1u, &none);
       }
       __syncwarp();
     }
@@ -476,6 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
   }
 
   // ---- products
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
   griddep_wait();                                  // row_exp
   griddep_launch_dependents();
   const int kw = warp % kSplit, mg = warp / kSplit, g = lane >> 2, t = lane & 3;
@@ -485,6 +587,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
   auto run = [&](const Task& w, auto nt_tag) {
     constexpr int NT = decltype(nt_tag)::value;
     const int m_first = own_first(w.m, mg), m_here = own_first(w.m, mg + 1) - m_first;
+    if ((int)threadIdx.x < w.cnt) s_exp[threadIdx.x] = __ldg(p.row_exp + w.r0 + threadIdx.x);   // for the end
     float sums[kM][NT][4];
 #pragma unroll
     for (int m = 0; m < kM; ++m)
@@ -494,14 +597,20 @@ __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
         for (int i = 0; i < 4; ++i) sums[m][nt][i] = 0.f;
 #pragma unroll 1
     for (int stage = 0; stage < p.stages; ++stage) {
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_full[slot], parity, &s_abort));
-      const uint8_t* at = s_mem + slot * kStage;
+      if (ok) ok = __all_sync(0xffffffffu, wait_for(&s_full[slot], parity, &s_abort));
+      const uint8_t* at = s_mem + slot * stage_bytes;
       const int left = p.k_steps - stage * kSplit, stride = (left < kSplit ? left : kSplit) * kRecord;
-      if (ok && m_here > 0 && kw < left)
-        multiply<T, NT, G, ZEROS>(at + m_first * stride + kw * kRecord, stride, m_here, at + kWeights, w.r0, kw, sums);
+      if (ok && kw < left) {
+        const uint8_t* records = at + m_first * stride + kw * kRecord;
+        const uint8_t* x = at + weights_bytes;
+        if (m_here == kM) multiply<T, NT, kM, G, ZEROS>(records, stride, x, kw, sums);
+        else if (m_here == 1) multiply<T, NT, 1, G, ZEROS>(records, stride, x, kw, sums);
+        else if (kM > 2 && m_here == 2) multiply<T, NT, 2, G, ZEROS>(records, stride, x, kw, sums);
+        else if (kM > 3 && m_here == 3) multiply<T, NT, 3, G, ZEROS>(records, stride, x, kw, sums);
+      }
       __syncwarp();
       if (lane == 0) mbar_arrive(&s_empty[slot]);
-      if (++slot == kStages) { slot = 0; parity ^= 1; }
+      if (++slot == stages) { slot = 0; parity ^= 1; }
     }
     // The warps' sums meet in shared memory and are added in the columns' order, 8 rows
     // of x at a time.
@@ -514,16 +623,17 @@ __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
         for (int i = 0; i < 4; ++i)
           mine[(2 * t + (i & 1)) * kSumStride + m * 16 + g + 8 * (i >> 1)] = sums[m][nt][i];
       named_bar_sync(1, kConsumers * 32);
-      for (int o = threadIdx.x; o < kGroupsM * 8 * kM * 16; o += kConsumers * 32) {
-        const int group = o / (8 * kM * 16), row = o / (kM * 16) % 8, n = o % (kM * 16);
-        const int tile = own_first(w.m, group) + n / 16, col = (w.m0 + tile) * 16 + n % 16;
-        if (tile >= own_first(w.m, group + 1) || nt * 8 + row >= w.cnt || col >= p.N) continue;
+#pragma unroll
+      for (int i = 0; i < kSumsEach; ++i) {
+        const int group = i * kConsumers * 32 / kGroupSums, n = (int)threadIdx.x % (kM * 16);
+        const int row = (i * kConsumers * 32 % kGroupSums + (int)threadIdx.x) / (kM * 16);
         float v = 0.f;
 #pragma unroll
         for (int q = 0; q < kSplit; ++q) v += s_sums[((group * kSplit + q) * 8 + row) * kSumStride + n];
-        const int r = w.r0 + nt * 8 + row;
-        v = ldexpf(v, 24 + __ldg(p.row_exp + r));
-        const size_t to = (size_t)r * p.N + col;
+        const int tile = own_first(w.m, group) + n / 16, in = nt * 8 + row, col = (w.m0 + tile) * 16 + n % 16;
+        if (tile >= own_first(w.m, group + 1) || in >= w.cnt || col >= p.N) continue;
+        v = ldexpf(v, (n & 8 ? 20 : 24) + s_exp[in]);          // rows g + 8 were 16 times theirs
+        const size_t to = (size_t)(w.r0 + in) * p.N + col;
         if (p.out_f32) static_cast<float*>(p.y)[to] = v;
         else static_cast<T*>(p.y)[to] = from_float<T>(v);
       }
@@ -558,14 +668,14 @@ uint64_t rows_bytes(int64_t R, int64_t d) { return (uint64_t)R * stages_of(d) * 
 
 template <typename T, int G, bool ZEROS>
 int launch_w4(const W4Params& p, const void* x, int d, int sms, cudaStream_t s) {
-  constexpr size_t kSmem = (size_t)kStages * (kTaskM * kSplit * record_bytes(G, ZEROS) + kMaxRows * kRowPiece) + kSumBytes;
-  static_assert(kSmem + 4 * (kMaxExperts + 4) + 1024 <= 227 * 1024, "shared memory");
+  static_assert(kSumsEach * kSplit == 4 * kM && kGroupSums % (kConsumers * 32) == 0, "sums are shared out evenly");
+  static_assert(2 * (kTaskM * kSplit * record_bytes(G, ZEROS) + kMaxRows * kRowPiece) + kSumBytes <= kSmem, "two stages");
   static std::atomic<void*> seen[kMaxCachedDevices];
   cudaError_t e = once_per_context(seen, [] {
     return cudaFuncSetAttribute(w4_kernel<T, G, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
   });
   if (e != cudaSuccess) return cuda_status(e);
-  e = launch_pdl(w4_rows_kernel<T>, dim3((p.R + 7) / 8), dim3(kRowsThreads), 0, s, static_cast<const T*>(x),
+  e = launch_pdl(w4_rows_kernel<T, G>, dim3(p.R), dim3(kRowsThreads), 0, s, static_cast<const T*>(x),
                  p.R, d, p.stages, const_cast<uint8_t*>(p.x), const_cast<int32_t*>(p.row_exp));
   if (e != cudaSuccess) return cuda_status(e);
   return cuda_status(launch_pdl(w4_kernel<T, G, ZEROS>, dim3(sms), dim3(kThreads), kSmem, s, p));
@@ -647,6 +757,8 @@ MOE_API int moe_w4_matvec(const void* x, const void* layout, const int32_t* offs
   p.n_tiles = (n + 15) / 16;
   p.k_steps = (d + kStepK - 1) / kStepK;
   p.stages = stages_of(d);
+  // whatever the offsets, (chunk, row of tiles) pairs are numbered in 32 bits
+  if ((int64_t)num_experts * ((num_rows + kMaxRows - 1) / kMaxRows) * p.n_tiles > INT32_MAX) return MOE_ERR_TOO_LARGE;
   p.x = static_cast<const uint8_t*>(workspace);
   p.row_exp = reinterpret_cast<const int32_t*>(p.x + rows_bytes(num_rows, d));
   p.records = static_cast<const uint8_t*>(layout);

@@ -337,7 +337,8 @@ MOE_API int moe_w4_lay_out(const void* codes, const void* scales, const void* ze
  * The rows go through the workspace (moe_w4_workspace_size bytes, 16-byte aligned, any
  * contents, not shared by calls that may overlap), bf16 ones scaled by a power of two
  * each into fp16: values more than 2^28 below the row's largest are off by at most
- * 2^-39 of that, others by nothing.  x is 16-byte aligned.                   */
+ * 2^-39 of that, others by nothing.  A row with an infinity or a NaN has no finite
+ * products.  x is 16-byte aligned.                                           */
 MOE_API int moe_w4_workspace_size(int32_t num_rows, int32_t d, uint64_t* bytes);
 MOE_API int moe_w4_matvec(const void* x, const void* layout, const int32_t* offsets, int32_t num_rows,
                           int32_t num_experts, int32_t n, int32_t d, int32_t group_size, int32_t with_zeros,

@@ -19,27 +19,31 @@ def make(E, N, D, group, zeros, dtype, dev, seed):
 
 
 def dense(codes, scales, zeros, group):
-    """fp64 weights [E, N, D]."""
+    """fp64 weights [E, N, D], and (code + zero) * |scale|: a product is made as sum of code * x minus zero *
+    (sum of x), so these are the magnitudes of the terms that are added."""
     q = torch.stack([codes & 15, codes >> 4], -1).flatten(-2).double()
     z = zeros.double().repeat_interleave(group, -1) if zeros is not None else 8.0
-    return (q - z) * scales.double().repeat_interleave(group, -1)
+    s = scales.double().repeat_interleave(group, -1)
+    return (q - z) * s, (q + z) * s.abs()
 
 
 def sum_error(D):
-    """Roundings on the way of a product to the output, in units of 2^-24 of the terms' sum: a tensor core
-    step adds 16 exact products and the sum so far with at least 24 bits each (17 units), at most 4 steps a
-    group and tile, then one for the scale, a chain over the tiles of a warp and of 8 warps."""
-    return 4 * 17 + (D // 64 + 8) // 8 + 8 + 4
+    """Roundings on the way of a product to the output, in units of 2^-24 of the terms' sum: the sum of x over a
+    group (8 values, then a tree over 16 threads) and its product with the zero point; a tensor core step adds
+    16 exact products and the sum so far with at least 24 bits each (17 units), at most 8 steps a group; then
+    one for the scale and its sum for each group of a quarter of the columns, and 4 quarters."""
+    return 7 + 4 + 1 + 8 * 17 + (D // 32 + 3) // 4 + 4 + 4
 
 
 def check(y, x, W, offsets, dtype, D):
     R = x.shape[0]
+    W, M = W
     ref = torch.zeros(R, W.shape[1], dtype=torch.float64, device=x.device)
     mag = torch.zeros_like(ref)
     for e in range(W.shape[0]):
         a, b = offsets[e], offsets[e + 1]
         ref[a:b] = x[a:b].double() @ W[e].t()
-        mag[a:b] = x[a:b].double().abs() @ W[e].abs().t()
+        mag[a:b] = x[a:b].double().abs() @ M[e].t()
     assert_close(y, ref, dtype, sum_error(D) * U32 * mag, "y")
 
 
@@ -115,9 +119,9 @@ def test_layout_is_the_documented_one(N, D, group, zeros, pkg, cuda_dev):
         assert torch.equal(part.reshape(E, n16 * 16, -1), full)
 
 
-def test_pruned_weights_and_small_values_are_exact(pkg, cuda_dev):
-    """Codes equal to their zero points give exact zeros, and a value far below its row's largest still counts
-    where the largest has no weight."""
+def test_pruned_weights_and_outliers(pkg, cuda_dev):
+    """Codes equal to their zero points, and a value far above its row's others that has no weight: within the
+    roundings of code * x and zero * x, which do not cancel exactly."""
     torch.manual_seed(0)
     N, D = 40, 256
     z = torch.randint(0, 16, (1, N, D // 32), device=cuda_dev, dtype=torch.uint8)
@@ -125,17 +129,19 @@ def test_pruned_weights_and_small_values_are_exact(pkg, cuda_dev):
     s = torch.rand(1, N, D // 32, device=cuda_dev).bfloat16() + 1
     x = torch.randn(3, D, device=cuda_dev).bfloat16() * 1000
     off = torch.tensor([0, 3], dtype=torch.int32, device=cuda_dev)
-    w = pkg.W4Weights(q[..., 0::2] | q[..., 1::2] << 4, s, z, group_size=32)
-    assert not bool(pkg.w4_matvec(x, w, off).any())
-    w = pkg.W4Weights(torch.full((1, N, D // 2), 0x88, dtype=torch.uint8, device=cuda_dev), s, group_size=32)
-    assert not bool(pkg.w4_matvec(x, w, off).any())
+    for codes, zeros in ((q[..., 0::2] | q[..., 1::2] << 4, z),
+                         (torch.full((1, N, D // 2), 0x88, dtype=torch.uint8, device=cuda_dev), None)):
+        w = pkg.W4Weights(codes, s, zeros, group_size=32)
+        W = dense(codes, s, zeros, 32)
+        assert not bool(W[0].any())
+        check(pkg.w4_matvec(x, w, off), x, W, [0, 3], torch.bfloat16, D)
     codes = torch.full((1, N, D // 2), 0x88, dtype=torch.uint8, device=cuda_dev)
     codes[0, :, 5] = 0x89                                       # column 10 counts once, column 11 not at all
     w = pkg.W4Weights(codes, s, group_size=32)
-    x = torch.zeros(1, D, device=cuda_dev).bfloat16()
-    x[0, 10], x[0, 11] = 1.5 * 2.0 ** -20, 2.0 ** 8
-    y = pkg.w4_matvec(x, w, off[:1].repeat(2) + torch.tensor([0, 1], device=cuda_dev, dtype=torch.int32))
-    assert torch.equal(y[0], (s[0, :, 0].float() * 1.5 * 2.0 ** -20).bfloat16())
+    for small in (2.0 ** -20, 2.0 ** -6, 1.0):
+        x = torch.zeros(1, D, device=cuda_dev).bfloat16()
+        x[0, 10], x[0, 11] = 1.5 * small, 2.0 ** 8
+        check(pkg.w4_matvec(x, w, out_dtype=torch.float32), x, dense(codes, s, None, 32), [0, 1], torch.float32, D)
 
 
 @pytest.mark.parametrize("size", [2.0 ** -126, 2.0 ** -60, 2.0 ** 60, 2.0 ** 120])
@@ -231,7 +237,7 @@ def test_moe_w4(T, K, total, E, first, H, I, dtype, pkg, cuda_dev):
     hidden, ids, weights, a, b = layer_inputs(T, K, total, E, first, H, I, dtype, cuda_dev)
     w13, w2 = (pkg.W4Weights(*m, group_size=32) for m in (a, b))
     out = pkg.moe_w4(hidden, ids, weights, w13, w2, first)
-    W13, W2 = dense(*a, 32), dense(*b, 32)
+    (W13, M13), (W2, M2) = dense(*a, 32), dense(*b, 32)
     u = torch.finfo(dtype).eps / 2
     ref = torch.zeros(T, H, dtype=torch.float64, device=cuda_dev)
     err = torch.zeros_like(ref)
@@ -241,7 +247,7 @@ def test_moe_w4(T, K, total, E, first, H, I, dtype, pkg, cuda_dev):
             if not 0 <= e < E:
                 continue
             h = hidden[t].double()
-            z, zm = W13[e] @ h, W13[e].abs() @ h.abs()
+            z, zm = W13[e] @ h, M13[e] @ h.abs()
             dz = z.abs() * u + sum_error(H) * U32 * zm + half_step(torch.zeros(1, device=cuda_dev).double(), dtype)
             up, gate, dup, dgate = z[:I], z[I:], dz[:I], dz[I:]
             s = up * gate * torch.sigmoid(gate)
@@ -250,7 +256,7 @@ def test_moe_w4(T, K, total, E, first, H, I, dtype, pkg, cuda_dev):
             ds = ds * (1 + u)
             w = float(weights[t, k])
             ref[t] += w * (W2[e] @ s)
-            err[t] += w * (W2[e].abs() @ (ds + sum_error(I) * U32 * (s.abs() + ds))) * (1 + K * 2 * U32)
+            err[t] += w * (W2[e].abs() @ ds + sum_error(I) * U32 * (M2[e] @ (s.abs() + ds))) * (1 + K * 2 * U32)
     err = err + K * 2 * U32 * ref.abs()
     assert_close(out, ref, dtype, err, "layer")
     given = torch.full_like(out, float("nan"))

@@ -84,7 +84,7 @@ def test_swiglu_and_w4_entries_check_their_arguments(pkg):
     assert lay(p + 2, p, None, 1, 16, 64, 32, p, None) == lay(p, p, None, 1, 16, 64, 32, p + 8, None) == odd
     size = lib.moe_w4_workspace_size
     assert size(-1, 128, ref) == size(4, 0, ref) == size(4, 128, None) == bad
-    assert size(4, 640, ref) == L.MOE_OK and n8.value == 4 * 2 * 1024 + 16
+    assert size(4, 640, ref) == L.MOE_OK and n8.value == 4 * 2 * 1088 + 16
     mv = lib.moe_w4_matvec
 
     def call(x=p, layout=p, offsets=p, R=4, E=2, n=16, d=128, group=64, dt=L.MOE_BF16, out=L.MOE_BF16, y=p, ws=256,
@@ -97,7 +97,7 @@ def test_swiglu_and_w4_entries_check_their_arguments(pkg):
     assert call(layout=None) == call(x=None) == call(y=None) == bad
     assert call(E=1025) == big
     assert call(x=p + 2) == call(layout=p + 8) == call(offsets=p + 2) == call(y=p + 1) == call(ws=264) == odd
-    assert call(ws=None) == call(nbytes=4 * 1024) == L.MOE_ERR_WORKSPACE_TOO_SMALL
+    assert call(ws=None) == call(nbytes=4 * 1088) == L.MOE_ERR_WORKSPACE_TOO_SMALL
     assert call(R=0, x=None, y=None) == L.MOE_OK
 
 
