@@ -57,7 +57,11 @@ constexpr int kThreads = (kConsumers + 4) * 32;     // a warpgroup beside them: 
 constexpr int kFewRegisters = 40, kManyRegisters = 232;
 constexpr int kMaxStages = 16;            // of the ring, as many as fit
 constexpr int kEarly = 4;                 // stages whose weights are copied before the rows of x are there
-constexpr int kMaxRows = 24;              // rows of x in a task
+// Rows of x in a task.  Four products of 8 rows side by side fit the registers except with
+// groups of 32, where they spill: 25 to 32 rows of all of 32 experts 264 us, in two tasks
+// 230 us (groups of 128: 211 and 267 us).
+__host__ __device__ constexpr int max_rows(int G) { return G == 32 ? 24 : 32; }
+constexpr int kMaxRows = 32;
 constexpr int kMaxExperts = 1024;
 constexpr int kStageK = kSplit * kStepK;  // columns of a stage
 constexpr int kRowPiece = kStageK * 2 + 64;   // bytes of a row of x in a stage: 512 fp16, then 16 sums of x
@@ -74,7 +78,7 @@ struct W4Params {
   const uint8_t* records;  // as above
   const int32_t* offsets;  // [E + 1], or null: one matrix for all rows
   void* y;
-  int R, N, E, n_tiles, k_steps, stages;
+  int R, N, E, n_tiles, k_steps, stages, max_rows;
   int out_f32, zero_rest;
 };
 
@@ -306,7 +310,7 @@ struct Tasks {
     }
     w.e = lo;
     int r;
-    const int rows = rows_of(*p, lo, &r), chunks = (rows + kMaxRows - 1) / kMaxRows, i = w.c - chunks_before[lo];
+    const int rows = rows_of(*p, lo, &r), chunks = (rows + p->max_rows - 1) / p->max_rows, i = w.c - chunks_before[lo];
     const int each = rows / chunks, more = rows - each * chunks;   // even chunks
     w.r0 = r + each * i + (i < more ? i : more);
     w.cnt = each + (i < more ? 1 : 0);
@@ -327,10 +331,10 @@ struct Tasks {
   }
 };
 // What a tile costs with this many rows of x, in sixths of the cost with 8: measured with all of 32
-// experts of 4096 x 7168 at 8, 16 and 24 rows (groups of 128: 92, 122, 162 us; of 32: 71, 115, 160).
+// experts of 4096 x 7168 at 8, 16 and 32 rows (groups of 128: 92, 122, 162 us; of 32: 71, 115, 160).
 template <int G>
 __device__ __forceinline__ int chunk_cost(int rows) {
-  return rows <= 8 ? 6 : rows <= 16 ? (G == 32 ? 9 : 8) : (G == 32 ? 13 : 11);
+  return rows <= 8 ? 6 : rows <= 16 ? (G == 32 ? 9 : 8) : rows <= 24 ? (G == 32 ? 13 : 11) : (G == 32 ? 16 : 14);
 }
 // The tiles of a task that a group of warps has: [own_first(m, group), own_first(m, group + 1)).
 __device__ __forceinline__ int own_first(int m, int group) { return m * group / kGroupsM; }
@@ -421,7 +425,7 @@ __device__ __forceinline__ void multiply(const uint8_t* records, int m_stride, c
 
 // A CTA of 8 warps that multiply (4 along the columns times 2 along the rows of tiles)
 // and one that copies.  A stage of the ring holds 4 steps of columns of up to 8 rows of tiles
-// and of up to 24 rows of x, about 60 KB in two or three copies (a copy for every
+// and of up to 32 rows of x, about 60 KB in two or three copies (a copy for every
 // row of tiles and of x made the copying warp the limit: 42 us of copies alone for 8
 // matrices of 4096 x 7168, the memory's rate being 19 us).
 template <typename T, int G, bool ZEROS>
@@ -447,10 +451,10 @@ __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
     fence_mbar_init();
   }
   __syncthreads();
-  // Chunks of up to kMaxRows rows before expert e: the same in every CTA.
+  // Chunks of up to max_rows rows before expert e: the same in every CTA.
   for (int e = threadIdx.x; e < p.E; e += kThreads) {
     int first;
-    const int rows = Tasks::rows_of(p, e, &first), chunks = (rows + kMaxRows - 1) / kMaxRows;
+    const int rows = Tasks::rows_of(p, e, &first), chunks = (rows + p.max_rows - 1) / p.max_rows;
     s_chunks[e] = chunks;
     if (chunks) atomicMax(&s_most_rows, (rows + chunks - 1) / chunks);
     s_cost[e] = chunks ? chunks * chunk_cost<G>((rows + chunks - 1) / chunks) : 0;
@@ -643,7 +647,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
   for (; work.m; tasks.next(work)) {
     if (work.cnt <= 8) run(work, std::integral_constant<int, 1>{});
     else if (work.cnt <= 16) run(work, std::integral_constant<int, 2>{});
-    else run(work, std::integral_constant<int, 3>{});
+    else if (work.cnt <= 24) run(work, std::integral_constant<int, 3>{});
+    else if constexpr (max_rows(G) > 24) run(work, std::integral_constant<int, 4>{});
   }
   if (!ok && lane == 0) raise_error(&g_w4_error, kDevTimeoutMma);
   if (p.zero_rest && p.offsets) {                  // rows of no expert
@@ -669,7 +674,8 @@ uint64_t rows_bytes(int64_t R, int64_t d) { return (uint64_t)R * stages_of(d) * 
 template <typename T, int G, bool ZEROS>
 int launch_w4(const W4Params& p, const void* x, int d, int sms, cudaStream_t s) {
   static_assert(kSumsEach * kSplit == 4 * kM && kGroupSums % (kConsumers * 32) == 0, "sums are shared out evenly");
-  static_assert(2 * (kTaskM * kSplit * record_bytes(G, ZEROS) + kMaxRows * kRowPiece) + kSumBytes <= kSmem, "two stages");
+  static_assert(2 * (kTaskM * kSplit * record_bytes(G, ZEROS) + max_rows(G) * kRowPiece) + kSumBytes <= kSmem,
+                "two stages");
   static std::atomic<void*> seen[kMaxCachedDevices];
   cudaError_t e = once_per_context(seen, [] {
     return cudaFuncSetAttribute(w4_kernel<T, G, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
@@ -758,7 +764,8 @@ MOE_API int moe_w4_matvec(const void* x, const void* layout, const int32_t* offs
   p.k_steps = (d + kStepK - 1) / kStepK;
   p.stages = stages_of(d);
   // whatever the offsets, (chunk, row of tiles) pairs are numbered in 32 bits
-  if ((int64_t)num_experts * ((num_rows + kMaxRows - 1) / kMaxRows) * p.n_tiles > INT32_MAX) return MOE_ERR_TOO_LARGE;
+  p.max_rows = max_rows(group_size);
+  if ((int64_t)num_experts * ((num_rows + p.max_rows - 1) / p.max_rows) * p.n_tiles > INT32_MAX) return MOE_ERR_TOO_LARGE;
   p.x = static_cast<const uint8_t*>(workspace);
   p.row_exp = reinterpret_cast<const int32_t*>(p.x + rows_bytes(num_rows, d));
   p.records = static_cast<const uint8_t*>(layout);

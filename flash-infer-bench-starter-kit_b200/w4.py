@@ -109,7 +109,7 @@ def w4_matvec(x: torch.Tensor, weights: W4Weights, offsets: torch.Tensor | None 
 
     ``x`` [R, D] has the weights' type; ``offsets`` int32 [E + 1] as ``sort_tokens`` gives them, None for a
     single matrix.  Rows outside ``[offsets[0], offsets[E])`` are zero in a new result and left as they
-    were in a given ``out``.  The weights of each expert with rows are read once for up to 24 rows, so
+    were in a given ``out``.  The weights of each expert with rows are read once for up to 32 rows, so
     this is the product for decode batches; prefill batches want a GEMM.  A row of ``x`` with an infinity or a
     NaN has no finite products."""
     if not isinstance(weights, W4Weights):

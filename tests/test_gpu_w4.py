@@ -50,7 +50,7 @@ def check(y, x, W, offsets, dtype, D):
 CASES = [  # E, N, D, group, rows of each expert
     (1, 64, 64, 64, [1]), (1, 1, 32, 32, [3]), (1, 4096, 7168, 128, [1]), (1, 17, 96, 32, [8]),
     (3, 100, 128, 128, [0, 9, 0]), (5, 130, 192, 64, [16, 0, 17, 1, 33]), (4, 2048, 416, 32, [2, 31, 32, 70]),
-    (40, 48, 256, 128, [1] * 40), (2, 7168, 2048, 128, [5, 24]), (3, 96, 640, 128, [25, 49, 23]), (3, 16, 1024, 64, [0, 0, 0]),
+    (40, 48, 256, 128, [1] * 40), (2, 7168, 2048, 128, [5, 24]), (3, 96, 640, 128, [25, 49, 23]), (2, 80, 384, 128, [32, 65]), (3, 16, 1024, 64, [0, 0, 0]),
     (300, 33, 64, 32, [i % 3 for i in range(300)]),
 ]
 
