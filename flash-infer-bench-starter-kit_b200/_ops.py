@@ -5,10 +5,13 @@ on the tensors' device and its current stream."""
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
 DTYPES = {torch.float32: _lib.MOE_F32, torch.float16: _lib.MOE_F16, torch.bfloat16: _lib.MOE_BF16}
+
+_entries: dict = {}
 
 
 def check_tensor(name, t, dtypes, shape, device):
@@ -18,9 +21,10 @@ def check_tensor(name, t, dtypes, shape, device):
         raise TypeError(f"{name} must be a torch.Tensor")
     if t.dtype not in dtypes:
         raise TypeError(f"{name} has dtype {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
-    if t.dim() != len(shape) or any(n != -1 and n != m for n, m in zip(shape, t.shape)):
+    got = t.shape
+    if len(got) != len(shape) or any(n != -1 and n != m for n, m in zip(shape, got)):
         want = ", ".join("any" if n == -1 else str(n) for n in shape)
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected ({want})")
+        raise ValueError(f"{name} has shape {tuple(got)}, expected ({want})")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor (no CPU path)")
     if device is not None and t.get_device() != device.index:
@@ -29,13 +33,24 @@ def check_tensor(name, t, dtypes, shape, device):
         raise ValueError(f"{name} must be contiguous")
 
 
+def differentiable_once(backward):
+    """``once_differentiable`` at no cost to ordinary backward passes, which run without gradients."""
+    marked = once_differentiable(backward)
+
+    def run(ctx, grad):
+        return (marked if torch.is_grad_enabled() else backward)(ctx, grad)
+    return run
+
+
 def call(name, device, *args):
-    """Run entry point ``name`` with ``args`` (tensors as pointers, None as NULL) on ``device``'s
+    """Run entry point ``name`` with ``args`` (pointers, None for NULL, and numbers) on ``device``'s
     current stream."""
-    fn = getattr(_lib.load(), name)
-    args = [a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args]
-    stream = torch.cuda.current_stream(device.index).cuda_stream
-    if torch.cuda.current_device() == device.index:
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(_lib.load(), name)
+    index = device.index
+    stream = torch.cuda.current_stream(index).cuda_stream
+    if torch.cuda.current_device() == index:
         status = fn(*args, stream)
     else:
         with torch.cuda.device(device):

@@ -8,9 +8,8 @@ products, and for training, it is a pass of its own.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from ._ops import DTYPES, call, check_tensor
+from ._ops import DTYPES, call, check_tensor, differentiable_once
 
 BLOCK = 128
 
@@ -22,18 +21,20 @@ class _Swiglu(torch.autograd.Function):
         y = torch.empty(R, I, dtype=x.dtype, device=x.device)
         codes = torch.empty(R, 2 * I, dtype=torch.float8_e4m3fn, device=x.device)
         scales = torch.empty(2 * -(-I // BLOCK), R, dtype=torch.float32, device=x.device)
-        call("moe_swiglu_forward", x.device, x, R, I, DTYPES[x.dtype], y, codes, scales)
+        call("moe_swiglu_forward", x.device, x.data_ptr(), R, I, DTYPES[x.dtype], y.data_ptr(), codes.data_ptr(),
+             scales.data_ptr())
         ctx.save_for_backward(codes, scales)
         return y
 
     @staticmethod
-    @once_differentiable
+    @differentiable_once
     def backward(ctx, grad_y):
         codes, scales = ctx.saved_tensors
         grad_y = grad_y.contiguous()
         R, I = grad_y.shape
         grad_x = torch.empty(R, 2 * I, dtype=grad_y.dtype, device=grad_y.device)
-        call("moe_swiglu_backward", grad_y.device, grad_y, codes, scales, R, I, DTYPES[grad_y.dtype], grad_x)
+        call("moe_swiglu_backward", grad_y.device, grad_y.data_ptr(), codes.data_ptr(), scales.data_ptr(), R, I,
+             DTYPES[grad_y.dtype], grad_x.data_ptr())
         return grad_x
 
 
@@ -53,5 +54,5 @@ def swiglu(x: torch.Tensor) -> torch.Tensor:
         return _Swiglu.apply(x)
     R, I = x.shape[0], x.shape[1] // 2
     y = torch.empty(R, I, dtype=x.dtype, device=x.device)
-    call("moe_swiglu_forward", x.device, x, R, I, DTYPES[x.dtype], y, None, None)
+    call("moe_swiglu_forward", x.device, x.data_ptr(), R, I, DTYPES[x.dtype], y.data_ptr(), None, None)
     return y

@@ -67,6 +67,7 @@ __device__ __forceinline__ void store_wide(T* p, const Pack<T, N>& x) {
   for (int i = 0; i < kBytes / kWord; ++i)
     *(reinterpret_cast<W*>(p) + i) = reinterpret_cast<const W*>(&x)[i];
 }
+template <> __device__ __forceinline__ uint8_t from_float(float v) { return (uint8_t)v; }   // for zeros
 template <typename T, int N>
 __device__ __forceinline__ Pack<T, N> zero_pack() {
   Pack<T, N> z;
@@ -74,6 +75,14 @@ __device__ __forceinline__ Pack<T, N> zero_pack() {
   for (int i = 0; i < N; ++i) z.v[i] = from_float<T>(0.f);
   return z;
 }
+
+// Asynchronous 16-byte copies to shared memory that bypass the L1 cache.
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 inline int dtype_bytes(int t) { return t == MOE_F32 ? 4 : t == MOE_F16 || t == MOE_BF16 ? 2 : 0; }
 

@@ -279,6 +279,209 @@ combine_backward_kernel(const TOut* __restrict__ grad_out, const TRow* __restric
   }
 }
 
+// --------------------------------------------------------------------------
+// The two kernels above for rows of whole 16-byte pieces and at most 8 picks, where
+// bandwidth counts.  With the rows in registers a thread needs 100 to 180 of them and too
+// few threads fit to cover the memory's latency (4096 tokens x 8 x 7168 bf16: combine 127,
+// its gradients 215 us).  Here every thread copies its own pieces of the next tokens
+// asynchronously into its own places in shared memory, kAhead steps ahead of the sums: no
+// registers, no barrier, and twice 256 threads x 2 steps x 128 bytes on their way on an SM.
+// --------------------------------------------------------------------------
+constexpr int kStreamThreads = 256, kSteps = 3;   // places for 3 steps: 2 ahead
+
+template <typename TRow, typename TOut, bool WEIGHTED>
+__global__ void __launch_bounds__(kStreamThreads, 2)
+combine_stream_kernel(const TRow* __restrict__ rows, const int32_t* __restrict__ inv_row,
+                      const float* __restrict__ weights, int T, int K, int nvec, TOut* __restrict__ out) {
+  constexpr int N = 16 / (int)sizeof(TRow);
+  extern __shared__ uint4 s_place[];               // [kSteps][kBatch][kStreamThreads]
+  griddep_wait();
+  griddep_launch_dependents();
+  const size_t H = (size_t)nvec * N;
+  const unsigned R = (unsigned)(T * K);
+  // Pieces (token, vector) are numbered through; a thread takes every stride-th.
+  const int stride = (int)gridDim.x * kStreamThreads, skip_t = stride / nvec, skip_v = stride - skip_t * nvec;
+  struct At {
+    int t, v;
+  };
+  auto next = [&](At& at) {
+    at.t += skip_t;
+    at.v += skip_v;
+    if (at.v >= nvec) {
+      at.v -= nvec;
+      ++at.t;
+    }
+  };
+  const int start = (int)blockIdx.x * kStreamThreads + (int)threadIdx.x;
+  At ahead = {start / nvec, start - start / nvec * nvec}, at = ahead;
+  int r[kBatch];                                   // of the next piece to copy
+  auto look_up = [&]() {
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) r[j] = ahead.t < T && j < K ? __ldg(inv_row + (size_t)ahead.t * K + j) : -1;
+  };
+  unsigned here[kSteps];                           // which picks' pieces are in a place
+  auto copy = [&](int place) {
+    here[place] = 0;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      if ((unsigned)r[j] < R) {
+        copy16(&s_place[(place * kBatch + j) * kStreamThreads + threadIdx.x], rows + (size_t)r[j] * H + (size_t)ahead.v * N);
+        here[place] |= 1u << j;
+      }
+    copies_commit();
+    next(ahead);
+    look_up();
+  };
+  look_up();
+#pragma unroll
+  for (int i = 0; i < kSteps - 1; ++i) copy(i);
+  while (at.t < T) {
+#pragma unroll
+    for (int place = 0; place < kSteps; ++place) {
+      copy((place + kSteps - 1) % kSteps);
+      if (at.t < T) {
+        float w[kBatch];
+        if (WEIGHTED) {
+#pragma unroll
+          for (int j = 0; j < kBatch; ++j) w[j] = j < K ? __ldg(weights + (size_t)at.t * K + j) : 0.f;
+        }
+        copies_wait<kSteps - 1>();
+        float acc[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          if (!(here[place] >> j & 1)) continue;
+          const uint4 raw = s_place[(place * kBatch + j) * kStreamThreads + threadIdx.x];
+          const Pack<TRow, N>& x = reinterpret_cast<const Pack<TRow, N>&>(raw);
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+            acc[i] = WEIGHTED ? fmaf(w[j], to_float(x.v[i]), acc[i]) : acc[i] + to_float(x.v[i]);
+        }
+        Pack<TOut, N> o;
+#pragma unroll
+        for (int i = 0; i < N; ++i) o.v[i] = from_float<TOut>(acc[i]);
+        store_wide<TOut, N>(out + (size_t)at.t * H + (size_t)at.v * N, o);
+      }
+      next(at);
+    }
+  }
+  copies_wait<0>();
+}
+
+// GS threads share a token and go over its vectors in steps.
+template <typename TRow, typename TOut, int GS>
+__global__ void __launch_bounds__(kStreamThreads, 2)
+combine_backward_stream_kernel(const TOut* __restrict__ grad_out, const TRow* __restrict__ rows,
+                               const int32_t* __restrict__ inv_row, const float* __restrict__ weights, int T, int K,
+                               int nvec, TRow* __restrict__ grad_rows, float* __restrict__ grad_weights) {
+  constexpr int N = 16 / (int)sizeof(TRow), kWarps = GS / 32, kGroups = kStreamThreads / GS;
+  extern __shared__ uint4 s_place[];               // [kSteps][kBatch][kStreamThreads]
+  __shared__ float s_dot[kGroups][kWarps][kBatch];
+  griddep_wait();
+  griddep_launch_dependents();
+  const size_t H = (size_t)nvec * N;
+  const unsigned R = (unsigned)(T * K);
+  const int group = (int)threadIdx.x / GS, lane = (int)threadIdx.x % GS;
+  const int first = (int)blockIdx.x * kGroups + group, stride = (int)gridDim.x * kGroups;
+  const int steps = (nvec + GS - 1) / GS;
+  struct At {
+    int t, step;
+  };
+  auto next = [&](At& at) {
+    if (++at.step < steps) return false;
+    at.step = 0;
+    at.t += stride;
+    return true;
+  };
+  At ahead = {first, 0}, at = ahead;
+  int r_ahead[kBatch], r[kBatch];
+  auto look_up = [&](int t, int (&rr)[kBatch]) {
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) rr[j] = t < T && j < K ? __ldg(inv_row + (size_t)t * K + j) : INT_MIN;
+  };
+  Pack<TOut, N> g[kSteps];
+  auto copy = [&](int place) {
+    const int v = ahead.step * GS + lane;
+    if (ahead.t < T && v < nvec) {
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if ((unsigned)r_ahead[j] < R)
+          copy16(&s_place[(place * kBatch + j) * kStreamThreads + threadIdx.x],
+                 rows + (size_t)r_ahead[j] * H + (size_t)v * N);
+      g[place] = load_stream<TOut, N>(grad_out + (size_t)ahead.t * H + (size_t)v * N);
+    }
+    copies_commit();
+    if (next(ahead)) look_up(ahead.t, r_ahead);
+  };
+  look_up(first, r_ahead);
+  float w[kBatch], dot[kBatch];
+  auto begin = [&]() {
+    look_up(at.t, r);
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      w[j] = at.t < T && j < K ? __ldg(weights + (size_t)at.t * K + j) : 0.f;
+      dot[j] = 0.f;
+    }
+  };
+  begin();
+#pragma unroll
+  for (int i = 0; i < kSteps - 1; ++i) copy(i);
+  while (at.t < T) {
+#pragma unroll
+    for (int place = 0; place < kSteps; ++place) {
+      copy((place + kSteps - 1) % kSteps);
+      copies_wait<kSteps - 1>();
+      const int v = at.step * GS + lane;
+      if (at.t < T && v < nvec) {
+        float gf[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) gf[i] = to_float(g[place].v[i]);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const unsigned row = r[j] >= 0 ? r[j] : -1 - r[j];
+          if (row >= R) continue;
+          Pack<TRow, N> o = zero_pack<TRow, N>();
+          if (r[j] >= 0) {
+            const uint4 raw = s_place[(place * kBatch + j) * kStreamThreads + threadIdx.x];
+            const Pack<TRow, N>& x = reinterpret_cast<const Pack<TRow, N>&>(raw);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              dot[j] = fmaf(gf[i], to_float(x.v[i]), dot[j]);
+              o.v[i] = from_float<TRow>(w[j] * gf[i]);
+            }
+          }
+          if (grad_rows) store_wide<TRow, N>(grad_rows + (size_t)row * H + (size_t)v * N, o);
+        }
+      }
+      const int t = at.t;
+      if (!next(at)) continue;                     // the same for a group's threads
+      // the token is done: its dot products over the group's threads
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+        for (int off = 16; off; off >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], off);
+      float mine = 0.f;
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if ((lane & 31) == j) mine = dot[j];
+      if (kWarps > 1) {
+        if ((lane & 31) < kBatch) s_dot[group][lane >> 5][lane & 31] = mine;
+        named_bar_sync(1 + group, GS);
+        if (lane < kBatch) {
+          mine = 0.f;
+#pragma unroll
+          for (int q = 0; q < kWarps; ++q) mine += s_dot[group][q][lane];
+        }
+        named_bar_sync(1 + group, GS);
+      }
+      if (t < T && lane < kBatch && lane < K) grad_weights[(size_t)t * K + lane] = mine;
+      begin();
+    }
+  }
+  copies_wait<0>();
+}
+
 // ---------------------------------------------------------------- host side
 // How many threads of a CTA lie along a row: the most (up to 256) that leave
 // the fewest lanes idle in the row's last chunk.
@@ -330,12 +533,61 @@ int run_combine_n(const void* rows, const int32_t* inv_row, const float* w, int 
                                 inv_row, w, T, K, H / N, g.chunks, g.tx, static_cast<TOut*>(out)));
 }
 
+constexpr size_t kPlaceBytes = (size_t)kSteps * kBatch * kStreamThreads * 16;
+
+// Two CTAs on each SM at most; fewer when there is less to do.
+int stream_grid(int64_t ctas, int* grid) {
+  int sms = 0;
+  const int st = require_device(&sms);
+  *grid = (int)(ctas < 2 * sms ? ctas : 2 * sms);
+  return st;
+}
+
+template <typename Kern, typename... Args>
+int launch_stream(std::atomic<void*>* seen, Kern kern, int grid, cudaStream_t s, Args... args) {
+  const cudaError_t e = once_per_context(seen, [&] {
+    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPlaceBytes);
+  });
+  if (e != cudaSuccess) return cuda_status(e);
+  return cuda_status(launch_pdl(kern, dim3(grid), dim3(kStreamThreads), kPlaceBytes, s, args...));
+}
+
+template <typename TRow, typename TOut>
+int run_combine_stream(const void* rows, const int32_t* inv_row, const float* w, int T, int K, int H, void* out,
+                       cudaStream_t s) {
+  static std::atomic<void*> seen[2][kMaxCachedDevices];
+  const int nvec = H / (16 / (int)sizeof(TRow));
+  int grid = 0;
+  const int st = stream_grid(((int64_t)T * nvec + kStreamThreads - 1) / kStreamThreads, &grid);
+  if (st != MOE_OK) return st;
+  if (w)
+    return launch_stream(seen[0], combine_stream_kernel<TRow, TOut, true>, grid, s, static_cast<const TRow*>(rows), inv_row,
+                         w, T, K, nvec, static_cast<TOut*>(out));
+  return launch_stream(seen[1], combine_stream_kernel<TRow, TOut, false>, grid, s, static_cast<const TRow*>(rows), inv_row, w,
+                       T, K, nvec, static_cast<TOut*>(out));
+}
+
+template <typename TRow, typename TOut, int GS>
+int run_backward_stream(const void* g, const void* rows, const int32_t* inv_row, const float* w, int T, int K, int H,
+                        void* grad_rows, float* grad_w, cudaStream_t s) {
+  static std::atomic<void*> seen[kMaxCachedDevices];
+  constexpr int kGroups = kStreamThreads / GS;
+  int grid = 0;
+  const int st = stream_grid((T + kGroups - 1) / kGroups, &grid);
+  if (st != MOE_OK) return st;
+  return launch_stream(seen, combine_backward_stream_kernel<TRow, TOut, GS>, grid, s, static_cast<const TOut*>(g),
+                       static_cast<const TRow*>(rows), inv_row, w, T, K, H / (16 / (int)sizeof(TRow)),
+                       static_cast<TRow*>(grad_rows), grad_w);
+}
+
 template <typename TRow, typename TOut>
 int run_combine(const void* rows, const int32_t* inv_row, const float* w, int T, int K, int H, void* out,
                 cudaStream_t s) {
   constexpr int kMost = 16 / (int)sizeof(TRow);
   int n = vector_elements(H, sizeof(TRow), kMost, {rows});
   n = vector_elements(H, sizeof(TOut), n, {out});
+  if (n == kMost && K <= kBatch && (int64_t)T * (H / n) < INT32_MAX / 2)
+    return run_combine_stream<TRow, TOut>(rows, inv_row, w, T, K, H, out, s);
   switch (n) {
     case 8: if constexpr (kMost >= 8) return run_combine_n<TRow, TOut, 8>(rows, inv_row, w, T, K, H, out, s);
     case 4: return run_combine_n<TRow, TOut, 4>(rows, inv_row, w, T, K, H, out, s);
@@ -368,6 +620,10 @@ int run_backward(const void* g, const void* rows, const int32_t* inv_row, const 
   constexpr int kMost = 16 / (int)sizeof(TRow);
   int n = vector_elements(H, sizeof(TRow), kMost, {grad_w ? rows : nullptr, grad_rows});
   n = vector_elements(H, sizeof(TOut), n, {g});
+  if (n == kMost && K <= kBatch && grad_w) {
+    if (H / n > 64) return run_backward_stream<TRow, TOut, 128>(g, rows, inv_row, w, T, K, H, grad_rows, grad_w, s);
+    return run_backward_stream<TRow, TOut, 32>(g, rows, inv_row, w, T, K, H, grad_rows, grad_w, s);
+  }
   switch (n) {
     case 8:
       if constexpr (kMost >= 8)

@@ -217,7 +217,8 @@ def read_device_error(device: torch.device | None = None) -> int:
     (and clear) their device error codes: the first non-zero one, or 0 when no device-side
     error happened since the last read.  The reads run on the current stream after it has
     waited on each workspace's last-use event, so streams the caller has destroyed since
-    are never touched."""
+    are never touched.  The 4-bit products' error word (one for the device) is read and
+    cleared with them, after the current stream's earlier work."""
     lib = _lib.load()
     idx = _device_index(device)
     with _ws_lock:
@@ -234,4 +235,10 @@ def read_device_error(device: torch.device | None = None) -> int:
                 _lib.check(st, "moe_fp8_ds_read_device_error")
             if first == 0:
                 first = int(code.value)
+        code = ctypes.c_int32(0)
+        st = lib.moe_w4_read_device_error(ctypes.c_void_p(cur.cuda_stream), ctypes.byref(code))
+        if st not in (_lib.MOE_OK, _lib.MOE_ERR_DEVICE_TIMEOUT):
+            _lib.check(st, "moe_w4_read_device_error")
+        if first == 0:
+            first = int(code.value)
     return first

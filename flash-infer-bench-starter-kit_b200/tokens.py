@@ -17,9 +17,8 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from ._ops import DTYPES, call, check_tensor
+from ._ops import DTYPES, call, check_tensor, differentiable_once
 
 
 class TokenOrder(NamedTuple):
@@ -43,7 +42,8 @@ def sort_tokens(topk_ids: torch.Tensor, num_local_experts: int, local_expert_off
     offsets = torch.empty(E + 1 if E > 0 else 1, dtype=torch.int32, device=dev)
     inv_row = torch.empty_like(topk_ids)
     row_token = torch.empty(T * K, dtype=torch.int32, device=dev)
-    call("moe_tokens_sort", dev, topk_ids, T, K, E, int(local_expert_offset), offsets, inv_row, row_token)
+    call("moe_tokens_sort", dev, topk_ids.data_ptr(), T, K, E, int(local_expert_offset), offsets.data_ptr(),
+         inv_row.data_ptr(), row_token.data_ptr())
     return TokenOrder(offsets, inv_row, row_token)
 
 
@@ -55,18 +55,20 @@ def _check_order(order, device):
 
 
 def _dispatch(hidden, inv_row):
-    T, K = inv_row.shape
-    rows = torch.empty(T * K, hidden.shape[1], dtype=hidden.dtype, device=hidden.device)
-    call("moe_tokens_dispatch", hidden.device, hidden, inv_row, T, K, hidden.shape[1], DTYPES[hidden.dtype], rows)
+    (T, K), H, dev = inv_row.shape, hidden.shape[1], hidden.device
+    rows = torch.empty(T * K, H, dtype=hidden.dtype, device=dev)
+    call("moe_tokens_dispatch", dev, hidden.data_ptr(), inv_row.data_ptr(), T, K, H, DTYPES[hidden.dtype],
+         rows.data_ptr())
     return rows
 
 
 def _combine(rows, weights, inv_row, out_dtype, out=None):
-    T, K = inv_row.shape
+    (T, K), H, dev = inv_row.shape, rows.shape[1], rows.device
     if out is None:
-        out = torch.empty(T, rows.shape[1], dtype=out_dtype, device=rows.device)
-    call("moe_tokens_combine", rows.device, rows, inv_row, weights, T, K, rows.shape[1], DTYPES[rows.dtype],
-         DTYPES[out_dtype], out)
+        out = torch.empty(T, H, dtype=out_dtype, device=dev)
+    call("moe_tokens_combine", dev, rows.data_ptr(), inv_row.data_ptr(),
+         None if weights is None else weights.data_ptr(), T, K, H, DTYPES[rows.dtype], DTYPES[out_dtype],
+         out.data_ptr())
     return out
 
 
@@ -77,7 +79,7 @@ class _Dispatch(torch.autograd.Function):
         return _dispatch(hidden, inv_row)
 
     @staticmethod
-    @once_differentiable
+    @differentiable_once
     def backward(ctx, grad_rows):
         inv_row, = ctx.saved_tensors
         return _combine(grad_rows.contiguous(), None, inv_row, grad_rows.dtype), None
@@ -92,7 +94,7 @@ class _Combine(torch.autograd.Function):
         return _combine(rows, weights, inv_row, out_dtype)
 
     @staticmethod
-    @once_differentiable
+    @differentiable_once
     def backward(ctx, grad_out):
         rows, weights, inv_row = ctx.saved_tensors
         shape, dtype = ctx.rows_like
@@ -100,8 +102,10 @@ class _Combine(torch.autograd.Function):
         dev = grad_out.device
         grad_rows = torch.empty(shape, dtype=dtype, device=dev) if ctx.needs_input_grad[0] else None
         grad_weights = torch.empty_like(weights) if ctx.needs_input_grad[1] else None
-        call("moe_tokens_combine_backward", dev, grad_out, rows, inv_row, weights, *inv_row.shape, shape[1],
-             DTYPES[dtype], DTYPES[grad_out.dtype], grad_rows, grad_weights)
+        call("moe_tokens_combine_backward", dev, grad_out.data_ptr(), None if rows is None else rows.data_ptr(),
+             inv_row.data_ptr(), weights.data_ptr(), *inv_row.shape, shape[1], DTYPES[dtype], DTYPES[grad_out.dtype],
+             None if grad_rows is None else grad_rows.data_ptr(),
+             None if grad_weights is None else grad_weights.data_ptr())
         return grad_rows, grad_weights, None, None
 
 

@@ -92,7 +92,8 @@ class W4Weights:
         zeros = zeros.contiguous() if zeros is not None else None
         if codes.data_ptr() % 4:
             codes = codes.clone()
-        call("moe_w4_lay_out", self.device, codes, scales, zeros, E, N, D, group_size, self.layout)
+        call("moe_w4_lay_out", self.device, codes.data_ptr(), scales.data_ptr(),
+             None if zeros is None else zeros.data_ptr(), E, N, D, group_size, self.layout.data_ptr())
 
 
 @functools.lru_cache(maxsize=4096)
@@ -136,9 +137,10 @@ def w4_matvec(x: torch.Tensor, weights: W4Weights, offsets: torch.Tensor | None 
         x = x.clone()
     need = _workspace_bytes(R, weights.d)
     workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    call("moe_w4_matvec", dev, x, weights.layout, offsets, R, weights.num_experts, weights.n, weights.d,
-         weights.group_size, int(weights.with_zeros), DTYPES[x.dtype], DTYPES[out.dtype], int(fresh), out, workspace,
-         need)
+    call("moe_w4_matvec", dev, x.data_ptr(), weights.layout.data_ptr(),
+         None if offsets is None else offsets.data_ptr(), R, weights.num_experts, weights.n, weights.d,
+         weights.group_size, int(weights.with_zeros), DTYPES[x.dtype], DTYPES[out.dtype], int(fresh), out.data_ptr(),
+         workspace.data_ptr(), need)
     return out
 
 

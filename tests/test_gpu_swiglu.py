@@ -93,7 +93,8 @@ def test_kept_codes_are_the_layers_activation_format(dtype, pkg, cuda_dev):
     y = torch.empty(R, I, dtype=dtype, device=cuda_dev)
     codes = torch.empty(R, 2 * I, dtype=torch.float8_e4m3fn, device=cuda_dev)
     scales = torch.empty(2 * I // BLOCK, R, device=cuda_dev)
-    ops.call("moe_swiglu_forward", x.device, x, R, I, ops.DTYPES[dtype], y, codes, scales)
+    ops.call("moe_swiglu_forward", x.device, x.data_ptr(), R, I, ops.DTYPES[dtype], y.data_ptr(), codes.data_ptr(),
+             scales.data_ptr())
     q, s = pkg.inputs.quant_rows_1x128(x.cpu().float())
     assert torch.equal(scales.cpu(), s)
     assert torch.equal(codes.cpu().view(torch.uint8), q.view(torch.uint8))

@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import sys
+
 import pytest
 import torch
 
@@ -215,6 +217,7 @@ def test_misaligned_rows_and_streams(pkg, cuda_dev):
             outs += [pkg.w4_matvec(x, w, off) for _ in range(5)]
     torch.cuda.synchronize()
     assert all(torch.equal(o, y) for o in outs)
+    assert sys.modules["fib_b200.kernel"].read_device_error(cuda_dev) == 0
 
 
 def layer_inputs(T, K, total, E, first, H, I, dtype, dev, group=32, zeros=True):
