@@ -25,6 +25,17 @@ template <> __device__ __forceinline__ float from_float(float v) { return v; }
 template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
 
+// Two values rounded to T, the first in the low half.
+template <typename T> __device__ __forceinline__ uint32_t two_of(float a, float b);
+template <> __device__ __forceinline__ uint32_t two_of<__half>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return reinterpret_cast<const uint32_t&>(v);
+}
+template <> __device__ __forceinline__ uint32_t two_of<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return reinterpret_cast<const uint32_t&>(v);
+}
+
 // N elements that are moved by as few accesses as their size allows.
 template <typename T, int N>
 struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Pack {

@@ -65,55 +65,89 @@ __device__ __forceinline__ void store_piece(T* p, int lane, int width, const flo
     const int c = column<N>(j, lane);
     if (c >= width) continue;
     Pack<T, N> x;
+    if constexpr (sizeof(T) == 2 && N >= 2) {    // two at a time: one instruction
 #pragma unroll
-    for (int i = 0; i < N; ++i) x.v[i] = from_float<T>(v[j * N + i]);
+      for (int i = 0; i < N; i += 2)
+        reinterpret_cast<uint32_t*>(&x)[i / 2] = two_of<T>(v[j * N + i], v[j * N + i + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x.v[i] = from_float<T>(v[j * N + i]);
+    }
     store_wide<T, N>(p + c, x);
   }
+}
+
+// Bits of the largest magnitude among a thread's columns (as fp32): a NaN's are above an
+// infinity's.  16-bit columns are compared two at a time.
+template <typename T> __device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b);   // signs are of no use
+template <> __device__ __forceinline__ uint32_t max_abs2<__nv_bfloat16>(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+template <> __device__ __forceinline__ uint32_t max_abs2<__half>(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+template <typename T, int N>
+__device__ __forceinline__ uint32_t largest(const Piece<T, N>& x, const float (&v)[kElems]) {
+  uint32_t bits = 0;
+  if constexpr (sizeof(T) == 2 && N >= 2) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&x);
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < kElems / 2; ++i) m = max_abs2<T>(m, w[i]);
+    m &= 0x7fff7fffu;
+    const Pack<T, 2> two = reinterpret_cast<const Pack<T, 2>&>(m);
+    bits = max(__float_as_uint(to_float(two.v[0])), __float_as_uint(to_float(two.v[1])));
+  } else {
+#pragma unroll
+    for (int i = 0; i < kElems; ++i) bits = max(bits, __float_as_uint(v[i]) & 0x7fffffffu);
+  }
+  return bits;
 }
 
 // v / s, correctly rounded, by Markstein's theorem (IBM Journal of Research and
 // Development 34, 1990): with r the correctly rounded 1 / s and q within a unit in the
 // last place of v / s, q + (v - q s) r rounds to the correctly rounded quotient, as long
-// as nothing leaves the range of normal numbers.  `plain` chooses the division itself for
-// scales near the ends of the range.  (32768 x 4096 bf16: 152 us with divisions.)
-__device__ __forceinline__ float2 quotients(float2 v, float s, float r, bool plain) {
-  if (plain) return make_float2(__fdiv_rn(v.x, s), __fdiv_rn(v.y, s));
+// as nothing leaves the range of normal numbers.  PLAIN is the division itself, for scales
+// near the ends of the range.  (32768 x 4096 bf16: 152 us with divisions.)
+template <bool PLAIN>
+__device__ __forceinline__ float2 quotients(float2 v, float s, float r) {
+  if (PLAIN) return make_float2(__fdiv_rn(v.x, s), __fdiv_rn(v.y, s));
   const float2 r2 = make_float2(r, r), q = __fmul2_rn(v, r2);
   const float2 left = __ffma2_rn(make_float2(-q.x, -q.y), make_float2(s, s), v);
   return __ffma2_rn(left, r2, q);
 }
 
-// Codes of a block and its scale (the same in all 16 lanes).
-template <int N>
-__device__ __forceinline__ float keep_block(uint8_t* q, int lane, int width, const float (&v)[kElems]) {
-  uint32_t bits = 0;                             // of the largest magnitude: a NaN's are above an infinity's
+template <int N, bool PLAIN>
+__device__ __forceinline__ void store_codes(uint8_t* q, int lane, int width, const float (&v)[kElems], float s, float r) {
+  auto two = [&](int i) {
+    return (uint32_t)__nv_cvt_float2_to_fp8x2(quotients<PLAIN>(make_float2(v[i], v[i + 1]), s, r), __NV_SATFINITE, __NV_E4M3);
+  };
 #pragma unroll
-  for (int i = 0; i < kElems; ++i) bits = max(bits, __float_as_uint(v[i]) & 0x7fffffffu);
+  for (int j = 0; j < kElems / N; ++j) {
+    const int c = column<N>(j, lane);
+    if (c >= width) continue;
+    if constexpr (N == 8) *reinterpret_cast<uint2*>(q + c) = make_uint2(two(0) | two(2) << 16, two(4) | two(6) << 16);
+    else if constexpr (N == 4) *reinterpret_cast<uint32_t*>(q + c) = two(4 * j) | two(4 * j + 2) << 16;
+    else if constexpr (N == 2) *reinterpret_cast<uint16_t*>(q + c) = (uint16_t)two(2 * j);
+    else q[c] = f32_to_e4m3(quotients<PLAIN>(make_float2(v[j], 0.f), s, r).x);
+  }
+}
+
+// Codes of a block and its scale (the same in all 16 lanes).
+template <typename T, int N>
+__device__ __forceinline__ float keep_block(uint8_t* q, int lane, int width, const Piece<T, N>& x, const float (&v)[kElems]) {
+  uint32_t bits = largest<T, N>(x, v);
 #pragma unroll
   for (int off = kLanes / 2; off; off >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, off));
   float s = __fdiv_rn(__uint_as_float(bits), kFp8Max);
   if (s == 0.f) s = 1.f;
   if (bits >= 0x7f800000u) s = __int_as_float(0x7fc00000);
-  const float r = __frcp_rn(s);
-  const bool plain = !(s > 0x1p-90f && s < 0x1p90f);
-#pragma unroll
-  for (int j = 0; j < kElems / N; ++j) {
-    const int c = column<N>(j, lane);
-    if (c >= width) continue;
-    if constexpr (N == 1) {
-      q[c] = f32_to_e4m3(quotients(make_float2(v[j], 0.f), s, r, plain).x);
-    } else {
-      Pack<uint8_t, N> o;
-#pragma unroll
-      for (int i = 0; i < N; i += 2) {
-        const float2 f = quotients(make_float2(v[j * N + i], v[j * N + i + 1]), s, r, plain);
-        const __nv_fp8x2_storage_t two = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
-        o.v[i] = (uint8_t)(two & 0xff);
-        o.v[i + 1] = (uint8_t)(two >> 8);
-      }
-      store_wide<uint8_t, N>(q + c, o);
-    }
-  }
+  if (s > 0x1p-90f && s < 0x1p90f) store_codes<N, false>(q, lane, width, v, s, __frcp_rn(s));
+  else store_codes<N, true>(q, lane, width, v, s, 0.f);
   return s;
 }
 
@@ -127,7 +161,7 @@ __device__ __forceinline__ void kept_values(const Piece<uint8_t, N>& q, float s,
     } else {
 #pragma unroll
       for (int i = 0; i < N; i += 2) {
-        const __nv_fp8x2_storage_t two = (__nv_fp8x2_storage_t)(q.v[j].v[i] | q.v[j].v[i + 1] << 8);
+        const __nv_fp8x2_storage_t two = reinterpret_cast<const __nv_fp8x2_storage_t*>(&q.v[j])[i / 2];
         const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3);
         const float2 f = __half22float2(__half2(h));
         v[j * N + i] = f.x * s;
@@ -141,7 +175,7 @@ __device__ __forceinline__ void kept_values(const Piece<uint8_t, N>& q, float s,
 // block, [2 * blocks][R]) are written as whole lines; neighbouring CTAs take
 // neighbouring blocks.  U rows are in flight in each thread.
 template <typename T, int N, int U, bool KEEP>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, KEEP ? 5 : 1)   // 32768 x 4096 bf16, kept: 117 us, unbounded 127 us
 swiglu_kernel(const T* __restrict__ x, int R, int I, int blocks, T* __restrict__ y, uint8_t* __restrict__ q,
               float* __restrict__ scale) {
   griddep_wait();
@@ -168,7 +202,7 @@ swiglu_kernel(const T* __restrict__ x, int R, int I, int blocks, T* __restrict__
     to_floats<T, N>(gate_in[u], gate);
     if constexpr (KEEP) {
       uint8_t* p = q + (size_t)r * 2 * I + col;
-      const float su = keep_block<N>(p, lane, w, up), sg = keep_block<N>(p + I, lane, w, gate);
+      const float su = keep_block<T, N>(p, lane, w, up_in[u], up), sg = keep_block<T, N>(p + I, lane, w, gate_in[u], gate);
       if (lane == 0 && r < R) {
         scale[(size_t)b * R + r] = su;
         scale[(size_t)(blocks + b) * R + r] = sg;

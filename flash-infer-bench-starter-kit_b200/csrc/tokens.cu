@@ -40,6 +40,8 @@ sort_kernel(const int32_t* __restrict__ ids, int P, int K, int E, int first, int
   int* s_hist = s_mem;                        // [warps][keys]: counts, then next rows
   int* s_total = s_mem + (size_t)warps * keys;   // [keys]: this CTA's counts
   int* s_start = s_total + keys;              // [keys]: first row of each key
+  int* s_before = s_start + keys;             // [keys]: counts of the CTAs before this one
+  __shared__ int s_warp[32];
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
   griddep_wait();
@@ -54,60 +56,97 @@ sort_kernel(const int32_t* __restrict__ ids, int P, int K, int E, int first, int
     const unsigned local = (unsigned)__ldg(ids + p) - (unsigned)first;   // wraps far above E when below first
     return local < (unsigned)E ? (int)local : E;
   };
-  for (int p = begin + lane; p < end; p += 32) atomicAdd(mine + key_of(p), 1);
+  constexpr int kTogether = 4;                // ids on their way at a time
+  for (int p0 = begin + lane; p0 < end; p0 += 32 * kTogether) {
+    int key[kTogether];
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) key[i] = p0 + 32 * i < end ? key_of(p0 + 32 * i) : -1;
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i)
+      if (key[i] >= 0) atomicAdd(mine + key[i], 1);
+  }
   __syncthreads();
-  for (int e = threadIdx.x; e < keys; e += blockDim.x) {   // counts -> offsets among this CTA's warps
+  // Counts to offsets among this CTA's warps: 4 threads a key, a quarter of the warps each.
+  for (int i = threadIdx.x; i < 4 * ((keys + 7) / 8 * 8); i += blockDim.x) {   // whole warps
+    const int e = i >> 2, quarter = warps / 4, w0 = (i & 3) * quarter;
     int sum = 0;
-    for (int w = 0; w < warps; ++w) {
-      const int c = s_hist[w * keys + e];
-      s_hist[w * keys + e] = sum;
-      sum += c;
+    if (e < keys)
+#pragma unroll 8
+      for (int w = w0; w < w0 + quarter; ++w) {
+        const int c = s_hist[w * keys + e];
+        s_hist[w * keys + e] = sum;
+        sum += c;
+      }
+    int incl = sum;
+#pragma unroll
+    for (int off = 1; off < 4; off <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, incl, off, 4);
+      if ((i & 3) >= off) incl += o;
     }
-    s_total[e] = sum;
+    if (e < keys) {
+      for (int w = w0; w < w0 + quarter; ++w) s_hist[w * keys + e] += incl - sum;
+      if ((i & 3) == 3) s_total[e] = incl;
+    }
   }
   if (ctas > 1) cluster.sync(); else __syncthreads();
-  for (int e = threadIdx.x; e < keys; e += blockDim.x) {   // offsets among the CTAs
+  // Offsets among the CTAs and, warp by warp, among the keys.
+  int carry = 0;                                           // of the keys of earlier rounds
+  for (int e0 = 0; e0 < keys; e0 += blockDim.x) {
+    const int e = e0 + (int)threadIdx.x;
     int before = 0, all = 0;
-    for (int c = 0; c < ctas; ++c) {
-      const int v = ctas > 1 ? cluster.map_shared_rank(s_total, c)[e] : s_total[e];
-      if (c < rank) before += v;
-      all += v;
-    }
-    s_start[e] = all;
-    for (int w = 0; w < warps; ++w) s_hist[w * keys + e] += before;
-  }
-  __syncthreads();
-  if (warp == 0) {                                         // offsets among the keys
-    int sum = 0;
-    for (int e0 = 0; e0 < keys; e0 += 32) {
-      const int e = e0 + lane, v = e < keys ? s_start[e] : 0;
-      int incl = v;
+    if (e < keys)
 #pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, incl, off);
-        if (lane >= off) incl += o;
+      for (int c = 0; c < kSortCluster; ++c) {
+        if (c >= ctas) break;
+        const int v = ctas > 1 ? cluster.map_shared_rank(s_total, c)[e] : s_total[e];
+        if (c < rank) before += v;
+        all += v;
       }
-      if (e < keys) s_start[e] = sum + incl - v;
-      sum += __shfl_sync(0xffffffffu, incl, 31);
+    int incl = all;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += o;
     }
+    if (lane == 31) s_warp[warp] = incl;
+    __syncthreads();
+    int base = carry;
+    for (int w = 0; w < warps; ++w) {
+      const int v = s_warp[w];
+      if (w < warp) base += v;
+      carry += v;
+    }
+    if (e < keys) {
+      s_start[e] = base + incl - all;
+      s_before[e] = before;
+    }
+    __syncthreads();
   }
-  __syncthreads();
   if (rank == 0)
     for (int e = threadIdx.x; e < keys; e += blockDim.x) offsets[e] = s_start[e];
   const int tail = s_start[E];
-  for (int p0 = begin; p0 < end; p0 += 32) {
-    const int p = p0 + lane;
-    const bool in = p < end;
-    const int key = in ? key_of(p) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, key);
-    if (in) {
-      const int row = s_start[key] + mine[key] + __popc(same & ((1u << lane) - 1u));
-      inv_row[p] = key < E ? row : -1 - row;
-      row_token[row] = row < tail ? p / K : -1;
+  for (int p0 = begin; p0 < end; p0 += 32 * kTogether) {
+    int key[kTogether];
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) {
+      const int p = p0 + 32 * i + lane;
+      key[i] = p < end ? key_of(p) : -1;
     }
-    __syncwarp();
-    if (in && lane == __ffs(same) - 1) mine[key] += __popc(same);
-    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) {
+      const int p = p0 + 32 * i + lane;
+      const unsigned same = __match_any_sync(0xffffffffu, key[i]);
+      int* next = mine + (key[i] < 0 ? 0 : key[i]);
+      const int at = *next;
+      __syncwarp();
+      if (key[i] >= 0) {
+        const int row = s_start[key[i]] + s_before[key[i]] + at + __popc(same & ((1u << lane) - 1u));
+        inv_row[p] = key[i] < E ? row : -1 - row;
+        row_token[row] = row < tail ? p / K : -1;
+        if (lane == __ffs(same) - 1) *next = at + __popc(same);
+      }
+      __syncwarp();
+    }
   }
   if (ctas > 1) cluster.sync();   // no CTA leaves while another still reads its counts
 }
@@ -621,6 +660,8 @@ int run_backward(const void* g, const void* rows, const int32_t* inv_row, const 
   int n = vector_elements(H, sizeof(TRow), kMost, {grad_w ? rows : nullptr, grad_rows});
   n = vector_elements(H, sizeof(TOut), n, {g});
   if (n == kMost && K <= kBatch && grad_w) {
+    // few tokens: all of a CTA's threads on each
+    if (H / n > 128 && T <= 256) return run_backward_stream<TRow, TOut, 256>(g, rows, inv_row, w, T, K, H, grad_rows, grad_w, s);
     if (H / n > 64) return run_backward_stream<TRow, TOut, 128>(g, rows, inv_row, w, T, K, H, grad_rows, grad_w, s);
     return run_backward_stream<TRow, TOut, 32>(g, rows, inv_row, w, T, K, H, grad_rows, grad_w, s);
   }
@@ -655,17 +696,17 @@ MOE_API int moe_tokens_sort(const int32_t* topk_ids, int32_t num_tokens, int32_t
     if (!aligned_to(p, 4)) return MOE_ERR_MISALIGNED;
   if ((st = require_device(nullptr)) != MOE_OK) return st;
   // One CTA for small batches; eight, as a cluster, when each of its warps
-  // would have more than four times 32 pairs.
-  const int ctas = P > 4096 ? kSortCluster : 1;
+  // would have more than 32 pairs (3885 pairs: 9.1 us with one, 7 with eight).
+  const int ctas = P > 1024 ? kSortCluster : 1;
   int threads = (P + 31) / 32 * 32;
-  threads = threads < 256 ? 256 : threads > 1024 ? 1024 : threads;
+  threads = threads < 256 ? 256 : threads > 1024 ? 1024 : (threads + 127) / 128 * 128;   // 4 warps or a multiple
   const int warps = threads / 32 * ctas;
   const int run = (int)((((int64_t)P + warps - 1) / warps + 31) / 32 * 32);
-  const size_t smem = ((size_t)(threads / 32) + 2) * (num_local_experts + 1) * sizeof(int);
+  const size_t smem = ((size_t)(threads / 32) + 3) * (num_local_experts + 1) * sizeof(int);
   static std::atomic<void*> seen[kMaxCachedDevices];
   cudaError_t e = once_per_context(seen, [] {
     return cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                (32 + 2) * (kSortMaxExperts + 1) * (int)sizeof(int));
+                                (32 + 3) * (kSortMaxExperts + 1) * (int)sizeof(int));
   });
   if (e != cudaSuccess) return cuda_status(e);
   cudaLaunchConfig_t cfg = {};
