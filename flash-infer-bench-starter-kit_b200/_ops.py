@@ -13,6 +13,11 @@ DTYPES = {torch.float32: _lib.MOE_F32, torch.float16: _lib.MOE_F16, torch.bfloat
 
 _entries: dict = {}
 
+# The handle of a device's current stream: torch's own accessor without a Stream object around it
+# where there is one (1.3 us of a 10 us call less).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
 
 def check_tensor(name, t, dtypes, shape, device):
     """``shape``: the expected sizes, -1 for any; ``dtypes``: the accepted types; ``device``: None
@@ -49,7 +54,7 @@ def call(name, device, *args):
     if fn is None:
         fn = _entries[name] = getattr(_lib.load(), name)
     index = device.index
-    stream = torch.cuda.current_stream(index).cuda_stream
+    stream = _raw_stream(index)
     if torch.cuda.current_device() == index:
         status = fn(*args, stream)
     else:
