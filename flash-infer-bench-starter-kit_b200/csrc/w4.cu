@@ -273,22 +273,29 @@ struct Tasks {
     *first = a;
     return b - a;
   }
-  // The pair (chunk, row of tiles), as chunk * n_tiles + tile, at which CTA b starts.
-  __device__ __forceinline__ int start_of(int b) const {
-    const int64_t at = (int64_t)cost_before[p->E] * p->n_tiles * b / (int)gridDim.x;
+  // Division of 64-bit numbers that mostly fit 32 bits.
+  static __device__ __forceinline__ uint64_t divide(uint64_t a, uint32_t b) {
+    return a >> 32 ? a / b : (uint64_t)((uint32_t)a / b);
+  }
+  // The pair (chunk, row of tiles), as chunk * n_tiles + tile, at which a run starts whose cost begins at `at`.
+  __device__ __forceinline__ int start_of(int64_t at) const {
     int lo = 0, hi = p->E;                                     // cost_before[lo] * n_tiles <= at
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if ((int64_t)cost_before[mid] * p->n_tiles <= at) lo = mid; else hi = mid;
     }
     const int chunks = chunks_before[lo + 1] - chunks_before[lo];
-    if (chunks <= 0) return chunks_before[p->E] * p->n_tiles;  // b is the number of CTAs
-    const int cost = (cost_before[lo + 1] - cost_before[lo]) / chunks;
-    const int tile = (int)((at - (int64_t)cost_before[lo] * p->n_tiles) / cost), most = chunks * p->n_tiles;
+    if (chunks <= 0) return chunks_before[p->E] * p->n_tiles;  // the end
+    const uint32_t cost = (uint32_t)(cost_before[lo + 1] - cost_before[lo]) / (uint32_t)chunks;
+    const int tile = (int)divide((uint64_t)(at - (int64_t)cost_before[lo] * p->n_tiles), cost), most = chunks * p->n_tiles;
     return chunks_before[lo] * p->n_tiles + (tile < most ? tile : most);
   }
   __device__ __forceinline__ Task begin() {
-    const int first = start_of(blockIdx.x), last = start_of(blockIdx.x + 1);
+    const int64_t total = (int64_t)cost_before[p->E] * p->n_tiles;
+    const int64_t each = (int64_t)divide((uint64_t)total, gridDim.x);
+    const uint32_t more = (uint32_t)(total - each * gridDim.x);
+    auto cost_at = [&](uint32_t b) { return each * b + more * b / gridDim.x; };
+    const int first = start_of(cost_at(blockIdx.x)), last = start_of(cost_at(blockIdx.x + 1));
     tiles = last - first;
     last_c = last / p->n_tiles;
     last_m = last - last_c * p->n_tiles;
@@ -441,14 +448,14 @@ __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
 
   // The kernel before this one, which has started, makes the rows of x; what came before
   // that one is complete, so the offsets and weights may be read.
+  if (threadIdx.x < kMaxStages) {
+    mbar_init(&s_full[threadIdx.x], 1);
+    mbar_init(&s_empty[threadIdx.x], kConsumers);
+    fence_mbar_init();
+  }
   if (threadIdx.x == 0) {
     s_abort = 0;
     s_most_rows = 0;
-    for (int i = 0; i < kMaxStages; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&s_empty[i], kConsumers);
-    }
-    fence_mbar_init();
   }
   __syncthreads();
   // Chunks of up to max_rows rows before expert e: the same in every CTA.
@@ -585,12 +592,15 @@ __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
   griddep_wait();                                  // row_exp
   griddep_launch_dependents();
   const int kw = warp % kSplit, mg = warp / kSplit, g = lane >> 2, t = lane & 3;
+  // With few tiles the groups of warps take turns at the stages instead of sharing out the tiles:
+  // one row of x and a matrix of 4096 x 7168, call after call, 13.9 -> 11.5 us.
+  const bool turns = tasks.most() <= kM;
   int slot = 0;
   uint32_t parity = 0;
   bool ok = true;                                  // after a wait that gave up: go on without work
   auto run = [&](const Task& w, auto nt_tag) {
     constexpr int NT = decltype(nt_tag)::value;
-    const int m_first = own_first(w.m, mg), m_here = own_first(w.m, mg + 1) - m_first;
+    const int m_first = turns ? 0 : own_first(w.m, mg), m_here = (turns ? w.m : own_first(w.m, mg + 1)) - m_first;
     if ((int)threadIdx.x < w.cnt) s_exp[threadIdx.x] = __ldg(p.row_exp + w.r0 + threadIdx.x);   // for the end
     float sums[kM][NT][4];
 #pragma unroll
@@ -604,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
       if (ok) ok = __all_sync(0xffffffffu, wait_for(&s_full[slot], parity, &s_abort));
       const uint8_t* at = s_mem + slot * stage_bytes;
       const int left = p.k_steps - stage * kSplit, stride = (left < kSplit ? left : kSplit) * kRecord;
-      if (ok && kw < left) {
+      if (ok && kw < left && (!turns || stage % kGroupsM == mg)) {
         const uint8_t* records = at + m_first * stride + kw * kRecord;
         const uint8_t* x = at + weights_bytes;
         if (m_here == kM) multiply<T, NT, kM, G, ZEROS>(records, stride, x, kw, sums);
@@ -634,8 +644,13 @@ __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
         float v = 0.f;
 #pragma unroll
         for (int q = 0; q < kSplit; ++q) v += s_sums[((group * kSplit + q) * 8 + row) * kSumStride + n];
-        const int tile = own_first(w.m, group) + n / 16, in = nt * 8 + row, col = (w.m0 + tile) * 16 + n % 16;
-        if (tile >= own_first(w.m, group + 1) || in >= w.cnt || col >= p.N) continue;
+        if (turns) {                               // what the other groups have of the same tiles
+          if (group) break;
+#pragma unroll
+          for (int q = kSplit; q < kConsumers; ++q) v += s_sums[(q * 8 + row) * kSumStride + n];
+        }
+        const int tile = (turns ? 0 : own_first(w.m, group)) + n / 16, in = nt * 8 + row, col = (w.m0 + tile) * 16 + n % 16;
+        if (tile >= (turns ? w.m : own_first(w.m, group + 1)) || in >= w.cnt || col >= p.N) continue;
         v = ldexpf(v, (n & 8 ? 20 : 24) + s_exp[in]);          // rows g + 8 were 16 times theirs
         const size_t to = (size_t)(w.r0 + in) * p.N + col;
         if (p.out_f32) static_cast<float*>(p.y)[to] = v;

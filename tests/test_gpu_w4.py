@@ -33,8 +33,8 @@ def sum_error(D):
     """Roundings on the way of a product to the output, in units of 2^-24 of the terms' sum: the sum of x over a
     group (8 values, then a tree over 16 threads) and its product with the zero point; a tensor core step adds
     16 exact products and the sum so far with at least 24 bits each (17 units), at most 8 steps a group; then
-    one for the scale and its sum for each group of a quarter of the columns, and 4 quarters."""
-    return 7 + 4 + 1 + 8 * 17 + (D // 32 + 3) // 4 + 4 + 4
+    one for the scale and its sum for each group of a quarter of the columns, and 4 quarters or 8 eighths."""
+    return 7 + 4 + 1 + 8 * 17 + (D // 32 + 3) // 4 + 4 + 8
 
 
 def check(y, x, W, offsets, dtype, D):
