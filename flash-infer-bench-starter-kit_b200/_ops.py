@@ -9,6 +9,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 
+INT32_MAX = 2 ** 31 - 1       # the library's sizes are 32-bit integers
 DTYPES = {torch.float32: _lib.MOE_F32, torch.float16: _lib.MOE_F16, torch.bfloat16: _lib.MOE_BF16}
 
 _entries: dict = {}
@@ -27,8 +28,8 @@ def check_tensor(name, t, dtypes, shape, device):
     if t.dtype not in dtypes:
         raise TypeError(f"{name} has dtype {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
     got = t.shape
-    if len(got) != len(shape) or any(n != -1 and n != m for n, m in zip(shape, got)):
-        want = ", ".join("any" if n == -1 else str(n) for n in shape)
+    if len(got) != len(shape) or any((n != -1 and n != m) or m > INT32_MAX for n, m in zip(shape, got)):
+        want = ", ".join(f"at most {INT32_MAX}" if n == -1 else str(n) for n in shape)
         raise ValueError(f"{name} has shape {tuple(got)}, expected ({want})")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor (no CPU path)")

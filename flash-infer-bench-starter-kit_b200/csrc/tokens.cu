@@ -689,6 +689,7 @@ MOE_API int moe_tokens_sort(const int32_t* topk_ids, int32_t num_tokens, int32_t
   if (st != MOE_OK) return st;
   if (num_local_experts < 1 || local_expert_offset < 0 || !offsets) return MOE_ERR_INVALID_ARGUMENT;
   if (num_local_experts > kSortMaxExperts) return MOE_ERR_TOO_LARGE;
+  if (local_expert_offset > INT32_MAX - num_local_experts) return MOE_ERR_TOO_LARGE;   // no id may wrap into the shard
   const int P = num_tokens * top_k;
   if (P > 0 && (!topk_ids || !inv_row || !row_token)) return MOE_ERR_INVALID_ARGUMENT;
   for (const void* p : {static_cast<const void*>(topk_ids), static_cast<const void*>(offsets),

@@ -771,16 +771,18 @@ MOE_API int moe_w4_matvec(const void* x, const void* layout, const int32_t* offs
       !aligned_to(y, dtype_bytes(out_dtype)) || !aligned_to(workspace, 16))
     return MOE_ERR_MISALIGNED;
   if (workspace_bytes < need || !workspace) return MOE_ERR_WORKSPACE_TOO_SMALL;
-  int sms = 0;
-  if ((st = require_device(&sms)) != MOE_OK) return st;
   W4Params p;
   p.R = num_rows; p.N = n; p.E = num_experts;
   p.n_tiles = (n + 15) / 16;
   p.k_steps = (d + kStepK - 1) / kStepK;
   p.stages = stages_of(d);
-  // whatever the offsets, (chunk, row of tiles) pairs are numbered in 32 bits
+  // whatever the offsets, (chunk, row of tiles) pairs and the chunks' costs (chunk_cost, at
+  // most 16) are numbered in 32 bits
   p.max_rows = max_rows(group_size);
-  if ((int64_t)num_experts * ((num_rows + p.max_rows - 1) / p.max_rows) * p.n_tiles > INT32_MAX) return MOE_ERR_TOO_LARGE;
+  const int64_t most_chunks = (int64_t)num_experts * (((int64_t)num_rows + p.max_rows - 1) / p.max_rows);
+  if (most_chunks * (p.n_tiles > 16 ? p.n_tiles : 16) > INT32_MAX) return MOE_ERR_TOO_LARGE;
+  int sms = 0;
+  if ((st = require_device(&sms)) != MOE_OK) return st;
   p.x = static_cast<const uint8_t*>(workspace);
   p.row_exp = reinterpret_cast<const int32_t*>(p.x + rows_bytes(num_rows, d));
   p.records = static_cast<const uint8_t*>(layout);

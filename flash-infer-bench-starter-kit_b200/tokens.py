@@ -18,7 +18,7 @@ from typing import NamedTuple
 
 import torch
 
-from ._ops import DTYPES, call, check_tensor, differentiable_once
+from ._ops import DTYPES, INT32_MAX, call, check_tensor, differentiable_once
 
 
 class TokenOrder(NamedTuple):
@@ -37,12 +37,14 @@ def sort_tokens(topk_ids: torch.Tensor, num_local_experts: int, local_expert_off
     T, K = topk_ids.shape
     if K < 1:
         raise ValueError("topk_ids needs at least one pick a token")
-    E = int(num_local_experts)
+    E, first = int(num_local_experts), int(local_expert_offset)
+    if E > INT32_MAX or abs(first) > INT32_MAX:
+        raise ValueError(f"experts {first} .. {first} + {E} are not numbered by int32 ids")
     dev = topk_ids.device
     offsets = torch.empty(E + 1 if E > 0 else 1, dtype=torch.int32, device=dev)
     inv_row = torch.empty_like(topk_ids)
     row_token = torch.empty(T * K, dtype=torch.int32, device=dev)
-    call("moe_tokens_sort", dev, topk_ids.data_ptr(), T, K, E, int(local_expert_offset), offsets.data_ptr(),
+    call("moe_tokens_sort", dev, topk_ids.data_ptr(), T, K, E, first, offsets.data_ptr(),
          inv_row.data_ptr(), row_token.data_ptr())
     return TokenOrder(offsets, inv_row, row_token)
 

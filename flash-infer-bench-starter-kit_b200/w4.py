@@ -19,7 +19,7 @@ import functools
 import torch
 
 from . import _lib
-from ._ops import DTYPES, call, check_tensor
+from ._ops import DTYPES, INT32_MAX, call, check_tensor
 from .activation import swiglu
 from .tokens import _combine, dispatch, sort_tokens
 
@@ -31,7 +31,7 @@ def quantize_w4(w: torch.Tensor, group_size: int, zero_points: bool = False, dty
     nearest of 16 values: codes uint8 [..., N, D / 2] (column 2j in the low half of byte j), scales
     ``dtype`` [..., N, D / group_size] and, with ``zero_points``, zeros uint8 of the same shape (the code
     that stands for 0; without, it is 8 and ``zeros`` is None)."""
-    if w.shape[-1] % group_size or group_size % 2:
+    if group_size < 2 or w.shape[-1] % group_size or group_size % 2:
         raise ValueError(f"{w.shape[-1]} columns do not split into groups of {group_size}")
     v = w.float().unflatten(-1, (-1, group_size))
     if zero_points:
@@ -73,7 +73,7 @@ class W4Weights:
             codes, scales = codes.unsqueeze(0), scales.unsqueeze(0)
             zeros = zeros.unsqueeze(0) if zeros is not None else None
         E, N, D = codes.shape[0], codes.shape[1], codes.shape[2] * 2
-        if E < 1 or N < 1 or D < 1 or D % group_size:
+        if E < 1 or N < 1 or D < 1 or D % group_size or max(E, N, D) > INT32_MAX:
             raise ValueError(f"codes of shape {tuple(codes.shape)} do not split into groups of {group_size} columns")
         for name, t in (("scales", scales), ("zeros", zeros)):
             if t is not None and t.shape != (E, N, D // group_size):
@@ -154,8 +154,8 @@ def moe_w4(hidden_states: torch.Tensor, topk_ids: torch.Tensor, topk_weights: to
             raise TypeError(f"{name} must be W4Weights")
     if w13.num_experts != w2.num_experts or w13.n != 2 * w2.d:
         raise ValueError(f"w13 has {w13.num_experts} experts of {w13.n} rows, w2 {w2.num_experts} of {w2.d} columns")
-    if hidden_states.requires_grad and torch.is_grad_enabled():
-        raise ValueError("moe_w4 has no gradient: detach hidden_states or call it under torch.no_grad()")
+    if (hidden_states.requires_grad or topk_weights.requires_grad) and torch.is_grad_enabled():
+        raise ValueError("moe_w4 has no gradient: detach its inputs or call it under torch.no_grad()")
     order = sort_tokens(topk_ids, w13.num_experts, local_expert_offset)
     T, K = topk_ids.shape
     check_tensor("topk_weights", topk_weights, (torch.float32,), (T, K), topk_ids.device)
@@ -165,4 +165,4 @@ def moe_w4(hidden_states: torch.Tensor, topk_ids: torch.Tensor, topk_weights: to
     rows = w4_matvec(dispatch(hidden_states, order), w13, order.offsets)
     # fp32 from the second product to the sum over k: one rounding, as in the fused layer
     down = w4_matvec(swiglu(rows), w2, order.offsets, out_dtype=torch.float32)
-    return _combine(down, topk_weights.detach(), order.inv_row, hidden_states.dtype, output)
+    return _combine(down, topk_weights, order.inv_row, hidden_states.dtype, output)

@@ -272,7 +272,8 @@ typedef enum moe_dtype {
  * t * K + k; pairs that are not on the shard come last in t * K + k order.
  * offsets int32 [E + 1] gives each expert's rows, inv_row int32 [T, K] a pair's
  * row, or -1 - row for a pair that is not on the shard, row_token int32 [T * K]
- * a row's token, -1 behind the last expert.  E <= 1024, T * K < 2^30.         */
+ * a row's token, -1 behind the last expert.  E <= 1024, T * K < 2^30,
+ * local_expert_offset + E < 2^31.                                            */
 MOE_API int moe_tokens_sort(const int32_t* topk_ids, int32_t num_tokens, int32_t top_k, int32_t num_local_experts,
                             int32_t local_expert_offset, int32_t* offsets, int32_t* inv_row, int32_t* row_token,
                             void* stream);
@@ -338,7 +339,7 @@ MOE_API int moe_w4_lay_out(const void* codes, const void* scales, const void* ze
  * contents, not shared by calls that may overlap), bf16 ones scaled by a power of two
  * each into fp16: values more than 2^28 below the row's largest are off by at most
  * 2^-39 of that, others by nothing.  A row with an infinity or a NaN has no finite
- * products.  x is 16-byte aligned.                                           */
+ * products.  x is 16-byte aligned.  E * ceil(R / 24) * max(n / 16, 16) < 2^31. */
 MOE_API int moe_w4_workspace_size(int32_t num_rows, int32_t d, uint64_t* bytes);
 MOE_API int moe_w4_matvec(const void* x, const void* layout, const int32_t* offsets, int32_t num_rows,
                           int32_t num_experts, int32_t n, int32_t d, int32_t group_size, int32_t with_zeros,

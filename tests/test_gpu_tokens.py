@@ -229,6 +229,26 @@ def test_streams_and_graph_replay(pkg, cuda_dev):
     torch.cuda.synchronize()
 
 
+def test_ids_at_the_ends_of_their_range(pkg, cuda_dev):
+    E = 5
+    first = 2 ** 31 - 1 - E
+    ids = torch.tensor([[first, INT_MIN], [INT_MIN + 1, 2 ** 31 - 2], [-1, 2 ** 31 - 1]], dtype=torch.int32, device=cuda_dev)
+    order = pkg.sort_tokens(ids, E, first)
+    for got, want in zip(order, order_on_host(ids.cpu(), E, first)):
+        assert torch.equal(got.cpu(), want)
+
+
+def test_no_second_derivative(pkg, cuda_dev):
+    """A gradient may be asked for with a graph of its own, but that graph has no gradient and says so."""
+    order = pkg.sort_tokens(torch.zeros(4, 1, dtype=torch.int32, device=cuda_dev), 2)
+    x = torch.randn(4, 16, device=cuda_dev, requires_grad=True)
+    w = torch.rand(4, 1, device=cuda_dev, requires_grad=True)
+    for y in (pkg.dispatch(x, order), pkg.combine(x, w, order), pkg.swiglu(x)):
+        first, = torch.autograd.grad((y * y).sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            first.sum().backward()
+
+
 def test_refusals(pkg, cuda_dev):
     L = __import__("sys").modules["fib_b200._lib"]
     ids = torch.zeros(4, 2, dtype=torch.int32, device=cuda_dev)
@@ -241,7 +261,10 @@ def test_refusals(pkg, cuda_dev):
         pkg.sort_tokens(ids.t(), 3)
     with pytest.raises(ValueError):
         pkg.sort_tokens(torch.zeros(4, 0, dtype=torch.int32, device=cuda_dev), 3)
-    for E, first in ((0, 0), (-1, 0), (1025, 0), (3, -1)):
+    for E, first in ((3, 2 ** 32), (2 ** 32 + 3, 0)):
+        with pytest.raises(ValueError):
+            pkg.sort_tokens(ids, E, first)
+    for E, first in ((0, 0), (-1, 0), (1025, 0), (3, -1), (3, 2 ** 31 - 3)):
         with pytest.raises(L.MoeError):
             pkg.sort_tokens(ids, E, first)
     x = torch.zeros(4, 16, device=cuda_dev)

@@ -297,6 +297,17 @@ def test_moe_w4_captured_twice(pkg, cuda_dev):
             assert torch.equal(out, pkg.moe_w4(hidden, ids, weights, w13, w2))
 
 
+def test_moe_w4_without_tokens_or_experts(pkg, cuda_dev):
+    hidden, ids, weights, m13, m2 = layer_inputs(5, 2, 8, 4, 0, 64, 32, torch.bfloat16, cuda_dev)
+    w13, w2 = pkg.W4Weights(*m13, group_size=32), pkg.W4Weights(*m2, group_size=32)
+    assert pkg.moe_w4(hidden[:0], ids[:0], weights[:0], w13, w2).shape == (0, 64)
+    out = torch.full_like(hidden, 3.0)
+    assert pkg.moe_w4(hidden, torch.full_like(ids, -1), weights, w13, w2, output=out) is out
+    assert not bool(out.any())
+    with pytest.raises(ValueError, match="gradient"):
+        pkg.moe_w4(hidden, ids, weights.clone().requires_grad_(True), w13, w2)
+
+
 def test_refusals(pkg, cuda_dev):
     codes, scales, _ = make(2, 32, 64, 32, False, torch.bfloat16, cuda_dev, 0)
     w = pkg.W4Weights(codes, scales, group_size=32)

@@ -34,6 +34,7 @@ def test_token_entries_check_their_arguments(pkg):
     assert sort(p, 4, 8, 4, -1, p, p, p, None) == bad
     assert sort(p, 4, 8, 1025, 0, p, p, p, None) == big
     assert sort(p, 1 << 27, 8, 4, 0, p, p, p, None) == big
+    assert sort(p, 4, 8, 4, 2 ** 31 - 4, p, p, p, None) == big     # ids would wrap into the shard
     assert sort(None, 4, 8, 4, 0, p, p, p, None) == bad
     assert sort(p, 4, 8, 4, 0, None, p, p, None) == bad
     assert sort(p, 4, 8, 4, 0, p, p + 2, p, None) == odd
@@ -96,6 +97,8 @@ def test_swiglu_and_w4_entries_check_their_arguments(pkg):
     assert call(dt=L.MOE_F32) == call(out=L.MOE_F16) == bad
     assert call(layout=None) == call(x=None) == call(y=None) == bad
     assert call(E=1025) == big
+    # 1024 * 131072 chunks of rows times 16
+    assert call(R=1 << 22, E=1024, n=1, nbytes=1 << 40) == big
     assert call(x=p + 2) == call(layout=p + 8) == call(offsets=p + 2) == call(y=p + 1) == call(ws=264) == odd
     assert call(ws=None) == call(nbytes=4 * 1088) == L.MOE_ERR_WORKSPACE_TOO_SMALL
     assert call(R=0, x=None, y=None) == L.MOE_OK
@@ -136,3 +139,19 @@ def test_quantize_w4_takes_the_nearest_value(zero_points, pkg):
     # half a step, and at an end of the range what the rounding of the scale (bf16, 2^-8) over 15 codes and
     # of the zero point (half a step) clips
     assert bool(((w - back).abs() <= step * (0.5 + 15 * 2.0 ** -8 + (0.5 if zero_points else 0.0))).all())
+
+
+def test_sizes_beyond_32_bits_are_refused(pkg):
+    """Not cut to 32 bits on their way into the library; meta tensors stand for the memory."""
+    def meta(*shape, dtype=torch.bfloat16):
+        return torch.empty(shape, dtype=dtype, device="meta")
+    much = 2 ** 31
+    for make in (lambda: pkg.sort_tokens(meta(much, 1, dtype=torch.int32), 4), lambda: pkg.swiglu(meta(much, 2)),
+                 lambda: pkg.swiglu(meta(1, 2 * much)),
+                 lambda: pkg.dispatch(meta(1, much), pkg.TokenOrder(*[meta(1, 1, dtype=torch.int32)] * 3))):
+        with pytest.raises(ValueError, match="2147483647"):
+            make()
+    with pytest.raises(ValueError, match="split"):
+        pkg.W4Weights(meta(1, much, 16, dtype=torch.uint8), meta(1, much, 1), group_size=32)
+    with pytest.raises(ValueError):
+        pkg.quantize_w4(torch.zeros(2, 4), 0)
