@@ -285,18 +285,24 @@ int run_backward_u(const void* dy, const void* q, const float* scale, int R, int
                                 static_cast<T*>(dx)));
 }
 
-// Rows in flight in a thread: kFlight where that still makes several CTAs for each SM.
+// Rows in flight in a thread: two where that still makes 8 CTAs for each SM and a thread's accesses
+// are of 16 bytes.  (us for the forward pass / the one that keeps codes / the backward
+// pass, two rows and one: 32768 x 4096 bf16 70 / 119 / 98 and 80 / 123 / 109; 512 x 4096 bf16
+// 8.2 / 10.2 / 8.2 and 8.2 / 8.2 / 8.2; single columns, 32768 x 2002 bf16, 51 / 96 / 90 and
+// 51 / 86 / 82; four, 32768 x 2008 bf16, 47 / 64 / 55 and 39 / 68 / 55.)
 constexpr int kFlight = 2;
 bool many_rows(int R, int I) { return swiglu_grid(R, I, kFlight).ctas >= 148 * 8; }
 
 template <typename T, int N>
 int run_forward(const void* x, int R, int I, void* y, void* q, float* scale, cudaStream_t s) {
-  if (many_rows(R, I)) return run_forward_u<T, N, kFlight>(x, R, I, y, q, scale, s);
+  if constexpr (N * sizeof(T) >= 16)
+    if (many_rows(R, I)) return run_forward_u<T, N, kFlight>(x, R, I, y, q, scale, s);
   return run_forward_u<T, N, 1>(x, R, I, y, q, scale, s);
 }
 template <typename T, int N>
 int run_backward(const void* dy, const void* q, const float* scale, int R, int I, void* dx, cudaStream_t s) {
-  if (many_rows(R, I)) return run_backward_u<T, N, kFlight>(dy, q, scale, R, I, dx, s);
+  if constexpr (N * sizeof(T) >= 16)
+    if (many_rows(R, I)) return run_backward_u<T, N, kFlight>(dy, q, scale, R, I, dx, s);
   return run_backward_u<T, N, 1>(dy, q, scale, R, I, dx, s);
 }
 

@@ -322,7 +322,7 @@ combine_backward_kernel(const TOut* __restrict__ grad_out, const TRow* __restric
 // The two kernels above for rows of whole 16-byte pieces and at most 8 picks, where
 // bandwidth counts.  With the rows in registers a thread needs 100 to 180 of them and too
 // few threads fit to cover the memory's latency (4096 tokens x 8 x 7168 bf16: combine 127,
-// its gradients 215 us).  Here every thread copies its own pieces of the next tokens
+// its gradients 215 us; with these 98 us, 5.4 TB/s, and 168 us, 5.9 TB/s).  Here every thread copies its own pieces of the next tokens
 // asynchronously into its own places in shared memory, kAhead steps ahead of the sums: no
 // registers, no barrier, and twice 256 threads x 2 steps x 128 bytes on their way on an SM.
 // --------------------------------------------------------------------------
@@ -625,7 +625,11 @@ int run_combine(const void* rows, const int32_t* inv_row, const float* w, int T,
   constexpr int kMost = 16 / (int)sizeof(TRow);
   int n = vector_elements(H, sizeof(TRow), kMost, {rows});
   n = vector_elements(H, sizeof(TOut), n, {out});
-  if (n == kMost && K <= kBatch && (int64_t)T * (H / n) < INT32_MAX / 2)
+  // From half a million pieces on the copies ahead pay (16-byte pieces of the output; bf16, 8 picks,
+  // us with and without: 8192 x 512 26.7 and 26.7, 4096 x 2048 39 and 43, 4096 x 7168 98 and 127;
+  // 64 x 1024 10.2 and 8.2).
+  const int64_t pieces = (int64_t)T * (H / n);
+  if (n == kMost && K <= kBatch && pieces >= 1 << 19 && pieces < INT32_MAX / 2)
     return run_combine_stream<TRow, TOut>(rows, inv_row, w, T, K, H, out, s);
   switch (n) {
     case 8: if constexpr (kMost >= 8) return run_combine_n<TRow, TOut, 8>(rows, inv_row, w, T, K, H, out, s);
@@ -660,9 +664,14 @@ int run_backward(const void* g, const void* rows, const int32_t* inv_row, const 
   int n = vector_elements(H, sizeof(TRow), kMost, {grad_w ? rows : nullptr, grad_rows});
   n = vector_elements(H, sizeof(TOut), n, {g});
   if (n == kMost && K <= kBatch && grad_w) {
-    // few tokens: all of a CTA's threads on each
-    if (H / n > 128 && T <= 256) return run_backward_stream<TRow, TOut, 256>(g, rows, inv_row, w, T, K, H, grad_rows, grad_w, s);
-    if (H / n > 64) return run_backward_stream<TRow, TOut, 128>(g, rows, inv_row, w, T, K, H, grad_rows, grad_w, s);
+    // A warp for each token needs no barriers, but its steps follow one another; so more threads for
+    // longer rows and for few tokens (bf16, us with 32 / 128 / 256 threads: 8192 x 1024, 8 picks,
+    // 59 / 67 / -, with 2 picks 33 / 45 / -; 2048 x 2048 33 / 35 / 39; 4096 x 7168 182 / 168 / 170;
+    // 512 x 1024 16 / 14 / -; 64 x 7168 55 / 21 / 14).
+    const int vectors = H / n;
+    if (vectors > 128 && T <= 256) return run_backward_stream<TRow, TOut, 256>(g, rows, inv_row, w, T, K, H, grad_rows, grad_w, s);
+    if (vectors > (T < 1024 ? 64 : 256))
+      return run_backward_stream<TRow, TOut, 128>(g, rows, inv_row, w, T, K, H, grad_rows, grad_w, s);
     return run_backward_stream<TRow, TOut, 32>(g, rows, inv_row, w, T, K, H, grad_rows, grad_w, s);
   }
   switch (n) {

@@ -15,8 +15,7 @@
 // What else was built and measured (us; 8 matrices of 4096 x 7168 times a row each /
 // 32 of them times 16 rows): zero points subtracted from the operands, 16 more
 // instructions for each 16 x 64 codes, 40 / 208; e4m3 operands, where a byte 0..15 is
-// q * 2^-9, 55 / 428 (mma.sync with e4m3 is converted to fp16 here, four times the
-// instructions); tcgen05.mma with the decoded weights in tensor memory, 112 / 410 (8
+// q * 2^-9, 55 / 428 (four times the executed instructions); tcgen05.mma with the decoded weights in tensor memory, 112 / 410 (8
 // products of N = 16 and their hand-overs took 2000 clocks for 128 x 128 codes that
 // arrive in 360).
 //
@@ -49,8 +48,7 @@ constexpr int kGroupsM = 2;               // groups of warps along the rows of t
 constexpr int kM = 4;                     // rows of tiles (of records) of a warp
 constexpr int kTaskM = kM * kGroupsM;     // of a task
 constexpr int kConsumers = kSplit * kGroupsM;       // warps that multiply
-constexpr int kSumsEach = 4 * kM / kSplit;          // sums a thread adds up for 8 rows of x
-constexpr int kGroupSums = 8 * kM * 16;             // of a group's tiles and 8 rows of x
+constexpr int kGroupSums = 8 * kM * 16;             // sums of a group's tiles and 8 rows of x
 constexpr int kThreads = (kConsumers + 4) * 32;     // a warpgroup beside them: one of its warps copies
 // Registers a thread: 168 at launch (384 threads share 64,512), then few for that
 // warpgroup and the rest for the two that multiply: 128 * 40 + 256 * 232 = 64,512.
@@ -61,12 +59,12 @@ constexpr int kEarly = 4;                 // stages whose weights are copied bef
 // groups of 32, where they spill: 25 to 32 rows of all of 32 experts 264 us, in two tasks
 // 230 us (groups of 128: 211 and 267 us).
 __host__ __device__ constexpr int max_rows(int G) { return G == 32 ? 24 : 32; }
-constexpr int kMaxRows = 32;
 constexpr int kMaxExperts = 1024;
 constexpr int kStageK = kSplit * kStepK;  // columns of a stage
 constexpr int kRowPiece = kStageK * 2 + 64;   // bytes of a row of x in a stage: 512 fp16, then 16 sums of x
 constexpr int kSumStride = kM * 16 + 4;   // of the sums in shared memory: a warp's stores hit 32 banks
-constexpr size_t kSumBytes = sizeof(float) * kConsumers * 8 * kSumStride;
+constexpr int kSumFloats = kConsumers * 8 * kSumStride;
+constexpr size_t kSumBytes = sizeof(float) * 2 * kSumFloats;   // two buffers
 constexpr size_t kSmem = 225 * 1024 - 8 * (kMaxExperts + 4);   // dynamic: the ring, then the sums
 
 // Bytes of a record with groups of G columns.
@@ -343,6 +341,7 @@ template <int G>
 __device__ __forceinline__ int chunk_cost(int rows) {
   return rows <= 8 ? 6 : rows <= 16 ? (G == 32 ? 9 : 8) : rows <= 24 ? (G == 32 ? 13 : 11) : (G == 32 ? 16 : 14);
 }
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 // The tiles of a task that a group of warps has: [own_first(m, group), own_first(m, group + 1)).
 __device__ __forceinline__ int own_first(int m, int group) { return m * group / kGroupsM; }
 
@@ -442,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
   __shared__ int s_chunks[kMaxExperts + 1], s_cost[kMaxExperts + 1];
   __shared__ __align__(8) uint64_t s_full[kMaxStages], s_empty[kMaxStages];
   __shared__ volatile int s_abort;
-  __shared__ int s_most_rows, s_exp[kMaxRows];
+  __shared__ int s_most_rows;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float* s_sums = reinterpret_cast<float*>(s_mem + (kSmem - kSumBytes));
 
@@ -595,13 +594,14 @@ __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
   // With few tiles the groups of warps take turns at the stages instead of sharing out the tiles:
   // one row of x and a matrix of 4096 x 7168, call after call, 13.9 -> 11.5 us.
   const bool turns = tasks.most() <= kM;
+  const int parties = turns ? kConsumers * 32 : kSplit * 32;   // threads that add up the same sums
+  int buffer = 0;
   int slot = 0;
   uint32_t parity = 0;
   bool ok = true;                                  // after a wait that gave up: go on without work
   auto run = [&](const Task& w, auto nt_tag) {
     constexpr int NT = decltype(nt_tag)::value;
     const int m_first = turns ? 0 : own_first(w.m, mg), m_here = (turns ? w.m : own_first(w.m, mg + 1)) - m_first;
-    if ((int)threadIdx.x < w.cnt) s_exp[threadIdx.x] = __ldg(p.row_exp + w.r0 + threadIdx.x);   // for the end
     float sums[kM][NT][4];
 #pragma unroll
     for (int m = 0; m < kM; ++m)
@@ -626,37 +626,42 @@ __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
       if (lane == 0) mbar_arrive(&s_empty[slot]);
       if (++slot == stages) { slot = 0; parity ^= 1; }
     }
-    // The warps' sums meet in shared memory and are added in the columns' order, 8 rows
-    // of x at a time.
-    float* mine = s_sums + warp * (8 * kSumStride);
+    // The sums of the warps that share tiles (a group, or all when they take turns) meet in shared
+    // memory and are added in the columns' order, 8 rows of x at a time.  A group waits for no
+    // other, so one adds up while another multiplies, and as the rounds take two buffers in turn, one
+    // barrier each is enough: who writes a buffer again has passed the barrier between, and by then
+    // all had read it.  (One buffer and all warps at both barriers: 2 to 9% more time.)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      float* mine = s_sums + buffer * kSumFloats + warp * (8 * kSumStride);
 #pragma unroll
       for (int m = 0; m < kM; ++m)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           mine[(2 * t + (i & 1)) * kSumStride + m * 16 + g + 8 * (i >> 1)] = sums[m][nt][i];
-      named_bar_sync(1, kConsumers * 32);
-#pragma unroll
-      for (int i = 0; i < kSumsEach; ++i) {
-        const int group = i * kConsumers * 32 / kGroupSums, n = (int)threadIdx.x % (kM * 16);
-        const int row = (i * kConsumers * 32 % kGroupSums + (int)threadIdx.x) / (kM * 16);
+      named_bar_sync(turns ? 1 : 2 + mg, parties);
+      const float* theirs = s_sums + buffer * kSumFloats + (turns ? 0 : mg * kSplit) * (8 * kSumStride);
+      buffer ^= 1;
+#pragma unroll 4
+      for (int i = (int)threadIdx.x % parties; i < kGroupSums; i += parties) {
+        const int n = i % (kM * 16), row = i / (kM * 16), tile = n / 16, in = nt * 8 + row;
+        const int col = (w.m0 + m_first + tile) * 16 + n % 16;
+        if (tile >= m_here || in >= w.cnt || col >= p.N) continue;
+        const int up = (n & 8 ? 20 : 24) + __ldg(p.row_exp + w.r0 + in);   // rows g + 8 were 16 times theirs
         float v = 0.f;
 #pragma unroll
-        for (int q = 0; q < kSplit; ++q) v += s_sums[((group * kSplit + q) * 8 + row) * kSumStride + n];
+        for (int q = 0; q < kSplit; ++q) v += theirs[(q * 8 + row) * kSumStride + n];
         if (turns) {                               // what the other groups have of the same tiles
-          if (group) break;
 #pragma unroll
-          for (int q = kSplit; q < kConsumers; ++q) v += s_sums[(q * 8 + row) * kSumStride + n];
+          for (int q = kSplit; q < kConsumers; ++q) v += theirs[(q * 8 + row) * kSumStride + n];
         }
-        const int tile = (turns ? 0 : own_first(w.m, group)) + n / 16, in = nt * 8 + row, col = (w.m0 + tile) * 16 + n % 16;
-        if (tile >= (turns ? w.m : own_first(w.m, group + 1)) || in >= w.cnt || col >= p.N) continue;
-        v = ldexpf(v, (n & 8 ? 20 : 24) + s_exp[in]);          // rows g + 8 were 16 times theirs
+        // v * 2^up, -100 <= up <= 138, in two factors of the same direction: no infinity on the way to a
+        // finite product, no rounding on the way to a normal one
+        v = v * power_of_two(up >> 1) * power_of_two(up - (up >> 1));
         const size_t to = (size_t)(w.r0 + in) * p.N + col;
         if (p.out_f32) static_cast<float*>(p.y)[to] = v;
         else static_cast<T*>(p.y)[to] = from_float<T>(v);
       }
-      named_bar_sync(1, kConsumers * 32);
     }
   };
   for (; work.m; tasks.next(work)) {
@@ -688,7 +693,6 @@ uint64_t rows_bytes(int64_t R, int64_t d) { return (uint64_t)R * stages_of(d) * 
 
 template <typename T, int G, bool ZEROS>
 int launch_w4(const W4Params& p, const void* x, int d, int sms, cudaStream_t s) {
-  static_assert(kSumsEach * kSplit == 4 * kM && kGroupSums % (kConsumers * 32) == 0, "sums are shared out evenly");
   static_assert(2 * (kTaskM * kSplit * record_bytes(G, ZEROS) + max_rows(G) * kRowPiece) + kSumBytes <= kSmem,
                 "two stages");
   static std::atomic<void*> seen[kMaxCachedDevices];

@@ -67,7 +67,7 @@ def misaligned(t):
 SHAPES = [  # T, K, total, E, first, H
     (1, 8, 256, 256, 0, 7168), (5, 3, 8, 8, 0, 1), (37, 8, 64, 64, 0, 1030), (64, 1, 16, 16, 0, 2048),
     (130, 12, 60, 30, 17, 257), (300, 5, 60, 60, 0, 96), (9, 4, 16, 4, 100, 512), (513, 2, 4, 2, 1, 1001),
-    (40, 8, 32, 16, 8, 4100),
+    (40, 8, 32, 16, 8, 4100), (4099, 8, 64, 32, 16, 1040), (8200, 3, 12, 12, 0, 520), (1100, 8, 8, 6, 1, 2048),
 ]
 
 
