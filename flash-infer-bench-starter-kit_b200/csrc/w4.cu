@@ -336,10 +336,12 @@ struct Tasks {
   }
 };
 // What a tile costs with this many rows of x, in sixths of the cost with 8: measured with all of 32
-// experts of 4096 x 7168 at 8, 16 and 32 rows (groups of 128: 92, 122, 162 us; of 32: 71, 115, 160).
+// experts at 8, 16, 24 and 32 rows less 10 us of start (4096 x 7168, groups of 128: 98, 124, 159 and
+// 198 us; 7168 x 2048, groups of 32: 75, 112 and 151 us, 25 to 32 rows being two chunks).  512 rows over
+// the 32 experts as a router leaves them: 175 us with 6, 8, 11, 14 here, 165 us with these.
 template <int G>
 __device__ __forceinline__ int chunk_cost(int rows) {
-  return rows <= 8 ? 6 : rows <= 16 ? (G == 32 ? 9 : 8) : rows <= 24 ? (G == 32 ? 13 : 11) : (G == 32 ? 16 : 14);
+  return rows <= 8 ? 6 : rows <= 16 ? (G == 32 ? 9 : 8) : rows <= 24 ? (G == 32 ? 12 : 10) : 12;
 }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 // The tiles of a task that a group of warps has: [own_first(m, group), own_first(m, group + 1)).
@@ -642,7 +644,6 @@ __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
       named_bar_sync(turns ? 1 : 2 + mg, parties);
       const float* theirs = s_sums + buffer * kSumFloats + (turns ? 0 : mg * kSplit) * (8 * kSumStride);
       buffer ^= 1;
-#pragma unroll 4
       for (int i = (int)threadIdx.x % parties; i < kGroupSums; i += parties) {
         const int n = i % (kM * 16), row = i / (kM * 16), tile = n / 16, in = nt * 8 + row;
         const int col = (w.m0 + m_first + tile) * 16 + n % 16;
