@@ -33,8 +33,9 @@
 //   8 * t + 4 * (j % 2) + {0, 2, 1, 3} in its bytes 0 to 3, row g in the low half of a
 //   byte and row g + 8 in the high half: a lane's share of x is then 16 consecutive
 //   bytes for each 32 columns;
-//   the record's scales [128 / G][8][2] (rows g, g + 8 together), then, if there are any,
-//   its zero points likewise.
+//   the record's scales [8][128 / G][2] (for row g of the first 8: group by group, row g's and
+//   row g + 8's together), then, if there are any, its zero points likewise: a lane's
+//   share of them is together.
 #include <type_traits>
 
 #include "rows.cuh"
@@ -132,11 +133,11 @@ w4_lay_out_kernel(const uint8_t* __restrict__ codes, const uint16_t* __restrict_
   } else {
     const int tail = piece - 64;
     const bool is_zeros = tail >= 2 * groups;
-    const int n = is_zeros ? 16 : 8, first = (is_zeros ? tail - 2 * groups : tail) * n;   // of the [groups][8][2] values
+    const int n = is_zeros ? 16 : 8, first = (is_zeros ? tail - 2 * groups : tail) * n;   // of the [8][groups][2] values
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       if (i >= n) break;
-      const int v = first + i, of = step * groups + v / 16, row = row0 + (v & 15) / 2 + 8 * (v & 1);
+      const int v = first + i, of = step * groups + v / 2 % groups, row = row0 + v / 2 / groups + 8 * (v & 1);
       if (row >= N || of * G >= D) continue;
       const size_t src = ((size_t)e * N + row) * (D / G) + of;
       if (is_zeros) o.b[i] = zeros[src];
@@ -373,6 +374,25 @@ __device__ __forceinline__ void multiply(const uint8_t* records, int m_stride, c
 #pragma unroll
       for (int part = 0; part < kParts; ++part) x_sum[nt][i][part] = v.v[part];
     }
+  // Scales and zero points come for the whole step together: with groups of 32 a row of each of 32
+  // experts of 7168 x 2048, with zero points, takes 77 us so and 81 with an access for each group.  With
+  // groups of 64 it takes more registers than there are (32 experts of 4096 x 7168 x 24 rows: 189 us so,
+  // 185 us group by group).
+  constexpr bool kTogether = kParts != 2;
+  Pack<uint32_t, kParts> scale[M];                 // of each group: row g's in the low half, row g + 8's
+  uint32_t zero[M][(kParts + 1) / 2];              // two groups a word, a byte for each of the rows
+#pragma unroll
+  for (int m = 0; kTogether && m < M; ++m) {
+    const uint8_t* tail = records + m * m_stride + 1024;
+    scale[m] = *reinterpret_cast<const Pack<uint32_t, kParts>*>(tail + g * kParts * 4);
+    if constexpr (ZEROS && kParts == 1) zero[m][0] = *reinterpret_cast<const uint16_t*>(tail + 32 + g * 2);
+    if constexpr (ZEROS && kParts > 1) {
+      using Words = Pack<uint32_t, kParts / 2>;
+      const Words v = *reinterpret_cast<const Words*>(tail + kParts * 32 + g * kParts * 2);
+#pragma unroll
+      for (int i = 0; i < kParts / 2; ++i) zero[m][i] = v.v[i];
+    }
+  }
   float a[M][NT][4];
   uint4 x[NT][2], codes[M];
 #pragma unroll
@@ -395,20 +415,26 @@ __device__ __forceinline__ void multiply(const uint8_t* records, int m_stride, c
       const uint32_t w = j % 4 == 0 ? codes[m].x : j % 4 == 1 ? codes[m].y : j % 4 == 2 ? codes[m].z : codes[m].w;
       const uint32_t w8 = w >> 8;
       const uint32_t a0 = w & 0x000f000fu, a1 = w & 0x00f000f0u, a2 = w8 & 0x000f000fu, a3 = w8 & 0x00f000f0u;
-      float z0 = 8.f, z1 = 128.f;                  // zero points, row g + 8's times 16 as its codes are
+      // Zero points z as the numbers 2^23 + z and, for row g + 8 whose codes are 16 times theirs,
+      // 2^27 + 16 * z: with -2^23 or -2^27 times the other factor added, an fma gives the product of z
+      // alone, rounded once.
+      float z0 = 0.f, z1 = 0.f;
       if (ZEROS && first) {
-        const uint32_t v =
-            *reinterpret_cast<const uint16_t*>(records + m * m_stride + 1024 + kParts * 32 + part * 16 + g * 2);
-        z0 = __uint_as_float(0x4b000000u | (v & 0xff)) - 8388608.f;
-        z1 = 16.f * (__uint_as_float(0x4b000000u | v >> 8) - 8388608.f);
+        if constexpr (!kTogether)
+          if (part == 0) zero[m][0] = *reinterpret_cast<const uint32_t*>(records + m * m_stride + 1024 + kParts * 32 + g * 4);
+        z0 = __uint_as_float(__byte_perm(zero[m][part / 2], 0x4b000000u, 0x7440 + part % 2 * 2));
+        z1 = __uint_as_float(__byte_perm(zero[m][part / 2], 0x4d000000u, 0x7441 + part % 2 * 2));
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const uint4 v = x[nt][j % 4 >> 1];
         const uint32_t b0 = (j & 1) ? v.z : v.x, b1 = (j & 1) ? v.w : v.y;
-        if (first)
-          mma_f16(a[m][nt], a0, a1, a2, a3, b0, b1, z0 * x_sum[nt][0][part], z0 * x_sum[nt][1][part],
-                  z1 * x_sum[nt][0][part], z1 * x_sum[nt][1][part]);
+        const float xs0 = x_sum[nt][0][part], xs1 = x_sum[nt][1][part];
+        if (first && ZEROS)
+          mma_f16(a[m][nt], a0, a1, a2, a3, b0, b1, fmaf(z0, xs0, -0x1p23f * xs0), fmaf(z0, xs1, -0x1p23f * xs1),
+                  fmaf(z1, xs0, -0x1p27f * xs0), fmaf(z1, xs1, -0x1p27f * xs1));
+        else if (first)
+          mma_f16(a[m][nt], a0, a1, a2, a3, b0, b1, 8.f * xs0, 8.f * xs1, 128.f * xs0, 128.f * xs1);
         else
           mma_f16(a[m][nt], a0, a1, a2, a3, b0, b1, a[m][nt][0], a[m][nt][1], a[m][nt][2], a[m][nt][3]);
       }
@@ -416,7 +442,9 @@ __device__ __forceinline__ void multiply(const uint8_t* records, int m_stride, c
     if (j % kWords != kWords - 1) continue;
 #pragma unroll
     for (int m = 0; m < M; ++m) {
-      const float2 s = pair_of<T>(*reinterpret_cast<const uint32_t*>(records + m * m_stride + 1024 + part * 32 + g * 4));
+      if constexpr (!kTogether)
+        scale[m].v[part] = *reinterpret_cast<const uint32_t*>(records + m * m_stride + 1024 + (g * kParts + part) * 4);
+      const float2 s = pair_of<T>(scale[m].v[part]);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

@@ -320,7 +320,7 @@ MOE_API int moe_swiglu_backward(const void* grad_y, const void* codes, const flo
  * d.  E <= 1024, d <= 2^24.  The layout: records of 16 rows x 128 columns (padding zero), [E][groups of
  * 8 records along n][stages of 4 records along d][8][4][record], where the last group and
  * the last stage hold what is left; a record is two 16 x 64 tiles of codes [32 lanes][16
- * bytes], then scales [128 / group_size][8][2] (rows g and g + 8 together), then zeros
+ * bytes], then scales [8][128 / group_size][2] (rows g and g + 8 together), then zeros
  * likewise if there are any.  Lane 4 * g + t of a tile holds, in bytes 0 to 3 of its 32-bit word j,
  * columns 32 * (j / 2) + 8 * t + 4 * (j % 2) + {0, 2, 1, 3} of row g (low half) and row g + 8
  * (high half).                                                               */

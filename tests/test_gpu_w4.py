@@ -117,7 +117,7 @@ def test_layout_is_the_documented_one(N, D, group, zeros, pkg, cuda_dev):
             continue
         full = torch.zeros(E, n16 * 16, steps * groups, dtype=plain.dtype)
         full[:, :N, :D // group] = plain.cpu()
-        part = part.reshape(E, n16, steps, groups, 8, 2).permute(0, 1, 5, 4, 2, 3)
+        part = part.reshape(E, n16, steps, 8, groups, 2).permute(0, 1, 5, 3, 2, 4)
         assert torch.equal(part.reshape(E, n16 * 16, -1), full)
 
 
