@@ -13,7 +13,7 @@
 // fp32; the factors 2^24 and 1/16 are left to the last step, and only the output is
 // rounded.
 // What else was built and measured (us; 8 matrices of 4096 x 7168 times a row each /
-// 32 of them times 16 rows): zero points subtracted from the operands, 16 more
+// 32 of them times 16 rows; this form 38 / 138): zero points subtracted from the operands, 16 more
 // instructions for each 16 x 64 codes, 40 / 208; e4m3 operands, where a byte 0..15 is
 // q * 2^-9, 55 / 428 (four times the executed instructions); tcgen05.mma with the decoded weights in tensor memory, 112 / 410 (8
 // products of N = 16 and their hand-overs took 2000 clocks for 128 x 128 codes that
@@ -459,6 +459,11 @@ __device__ __forceinline__ void multiply(const uint8_t* records, int m_stride, c
   }
 }
 
+// Measured, 32 experts of 4096 x 7168 in groups of 128, rows for each: 8 107 us (69% of the memory's
+// rate), 16 138, 24 173, 32 212.  Up to 8 rows memory and the copies' start bound it; beyond, the
+// products do: an mma.sync holds a scheduler for 8 clocks (2.0 an SM, measured), and the 4 to 10 other
+// instructions that each comes with (5 of them decode 8 codes for all rows) hardly overlap with it.
+//
 // A CTA of 8 warps that multiply (4 along the columns times 2 along the rows of tiles)
 // and one that copies.  A stage of the ring holds 4 steps of columns of up to 8 rows of tiles
 // and of up to 32 rows of x, about 60 KB in two or three copies (a copy for every

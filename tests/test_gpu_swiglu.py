@@ -12,7 +12,7 @@ from rounding import U32, assert_close
 pytestmark = pytest.mark.gpu
 
 BLOCK = 128
-SIZES = [(1, 2048), (3, 1), (5, 7), (17, 128), (64, 136), (33, 129), (250, 1000), (1000, 2048), (129, 516)]
+SIZES = [(1, 2048), (3, 1), (5, 7), (17, 128), (64, 136), (33, 129), (250, 1000), (1000, 2048), (129, 516), (4099, 1288)]
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
 
 
