@@ -5,6 +5,7 @@ on the tensors' device and its current stream."""
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -20,6 +21,14 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+def refuse_tangent(name, t):
+    """Refuse a dual tensor of forward-mode differentiation.  It need not require a gradient, so no
+    ``autograd.Function`` would see it, and its tangent would be lost without a word.  ``unpack_dual``
+    takes 0.7 us, so it is asked only while a dual level is open."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} carries a tangent: there is no forward-mode derivative")
+
+
 def check_tensor(name, t, dtypes, shape, device):
     """``shape``: the expected sizes, -1 for any; ``dtypes``: the accepted types; ``device``: None
     for any CUDA device."""
@@ -31,6 +40,7 @@ def check_tensor(name, t, dtypes, shape, device):
     if len(got) != len(shape) or any((n != -1 and n != m) or m > INT32_MAX for n, m in zip(shape, got)):
         want = ", ".join(f"at most {INT32_MAX}" if n == -1 else str(n) for n in shape)
         raise ValueError(f"{name} has shape {tuple(got)}, expected ({want})")
+    refuse_tangent(name, t)
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor (no CPU path)")
     if device is not None and t.get_device() != device.index:

@@ -19,7 +19,7 @@ import functools
 import torch
 
 from . import _lib
-from ._ops import DTYPES, INT32_MAX, call, check_tensor
+from ._ops import DTYPES, INT32_MAX, call, check_tensor, refuse_tangent
 from .activation import swiglu
 from .tokens import _combine, dispatch, sort_tokens
 
@@ -69,6 +69,7 @@ class W4Weights:
                 raise TypeError(f"{name} has dtype {t.dtype}, expected {' or '.join(str(d) for d in dtypes)}")
             if t.dim() not in (2, 3) or t.dim() != codes.dim() or t.device != codes.device:
                 raise ValueError(f"{name} must be [E, N, ...] or [N, ...], as and where the codes are")
+            refuse_tangent(name, t)
         if codes.dim() == 2:
             codes, scales = codes.unsqueeze(0), scales.unsqueeze(0)
             zeros = zeros.unsqueeze(0) if zeros is not None else None
