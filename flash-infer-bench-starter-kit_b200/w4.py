@@ -30,16 +30,24 @@ def quantize_w4(w: torch.Tensor, group_size: int, zero_points: bool = False, dty
     """``(codes, scales, zeros)`` of weights ``w`` [..., N, D], each group of ``group_size`` columns to the
     nearest of 16 values: codes uint8 [..., N, D / 2] (column 2j in the low half of byte j), scales
     ``dtype`` [..., N, D / group_size] and, with ``zero_points``, zeros uint8 of the same shape (the code
-    that stands for 0; without, it is 8 and ``zeros`` is None)."""
+    that stands for 0; without, it is 8 and ``zeros`` is None).  A scale that ``dtype`` cannot hold (fp16 ends
+    at 65504), or one of an infinity or a NaN, is refused, which waits for the GPU."""
     if group_size < 2 or w.shape[-1] % group_size or group_size % 2:
         raise ValueError(f"{w.shape[-1]} columns do not split into groups of {group_size}")
     v = w.float().unflatten(-1, (-1, group_size))
     if zero_points:
         low, high = v.amin(-1).clamp_max(0), v.amax(-1).clamp_min(0)
-        scales = ((high - low) / 15).to(dtype)
+        wanted = (high / 2 - low / 2) / 7.5                # high - low may leave fp32
     else:
-        scales = (v.abs().amax(-1) / 7).to(dtype)
-    scales = torch.where(scales > 0, scales, torch.ones_like(scales))
+        wanted = v.abs().amax(-1) / 7
+    # Below the type's normal numbers, where its steps are no longer small, a scale is rounded up: down, the
+    # group's ends would be clipped, or all of it lost with a scale of 0.
+    info = torch.finfo(dtype)
+    step = info.smallest_normal * info.eps
+    wanted = torch.where(wanted < info.smallest_normal, (torch.ceil(wanted.double() / step) * step).float(), wanted)
+    scales = torch.where(wanted == 0, torch.ones_like(wanted), wanted).to(dtype)
+    if not bool(torch.isfinite(scales).all()):
+        raise ValueError(f"weights whose scales are not finite in {dtype}")
     s = scales.float()
     zeros = torch.round(-low / s).clamp(0, 15) if zero_points else torch.full_like(s, 8)
     q = (torch.round(v / s.unsqueeze(-1)) + zeros.unsqueeze(-1)).clamp(0, 15).to(torch.uint8).flatten(-2)
