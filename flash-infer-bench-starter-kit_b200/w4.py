@@ -7,7 +7,8 @@ weights with group scales halve what its FP8 experts read:
     y   = w4_matvec(rows, w13, order.offsets)     # rows sorted by expert (sort_tokens, dispatch)
     out = moe_w4(hidden_states, topk_ids, topk_weights, w13, w2)       # the whole routed layer
 
-For inference only: there is no gradient.  The reference has no weights below
+For inference only: there is no gradient (``quantize_w4`` takes trained
+parameters, and leaves no graph behind).  The reference has no weights below
 8 bits.
 """
 
@@ -26,6 +27,7 @@ from .tokens import _combine, dispatch, sort_tokens
 GROUP_SIZES = (32, 64, 128)
 
 
+@torch.no_grad()
 def quantize_w4(w: torch.Tensor, group_size: int, zero_points: bool = False, dtype: torch.dtype = torch.bfloat16):
     """``(codes, scales, zeros)`` of weights ``w`` [..., N, D], each group of ``group_size`` columns to the
     nearest of 16 values: codes uint8 [..., N, D / 2] (column 2j in the low half of byte j), scales

@@ -72,3 +72,12 @@ def test_scales_that_are_not_finite_are_refused(zero_points, pkg):
             v[1, 40] = 15.0 * 65536
         with pytest.raises(ValueError, match="not finite"):
             pkg.quantize_w4(v, 32, zero_points, dtype)
+
+
+@pytest.mark.parametrize("zero_points", [False, True])
+def test_parameters_leave_no_graph_behind(zero_points, pkg):
+    """Quantised weights have no gradient, and must not hold a graph with fp32 copies of the parameter."""
+    w = torch.nn.Parameter(torch.randn(4, 64, generator=torch.Generator().manual_seed(1)))
+    got, want = pkg.quantize_w4(w, 32, zero_points), pkg.quantize_w4(w.detach(), 32, zero_points)
+    for a, b in zip(got, want):
+        assert (a is None and b is None) or (torch.equal(a, b) and not a.requires_grad)
