@@ -69,7 +69,7 @@ EXPORTS = (
     "moe_fp8_ds_last_cuda_error_string",
     "moe_tokens_sort", "moe_tokens_dispatch", "moe_tokens_combine", "moe_tokens_combine_backward",
     "moe_swiglu_forward", "moe_swiglu_backward", "moe_w4_layout_size", "moe_w4_lay_out",
-    "moe_w4_workspace_size", "moe_w4_matvec", "moe_w4_read_device_error",
+    "moe_w4_workspace_size", "moe_w4_matvec", "moe_w4_read_device_error", "moe_w4_selftest_ring",
 )
 
 _lib = None
@@ -125,6 +125,7 @@ def load() -> ctypes.CDLL:
         lib.moe_w4_layout_size.argtypes = [I32, I32, I32, I32, I32, ctypes.POINTER(U64)]
         lib.moe_w4_lay_out.argtypes = [P, P, P, I32, I32, I32, I32, P, P]
         lib.moe_w4_workspace_size.argtypes = [I32, I32, ctypes.POINTER(U64)]
+        lib.moe_w4_selftest_ring.argtypes = [P, I32, I32, P, P]
         lib.moe_w4_read_device_error.argtypes = [P, ctypes.POINTER(I32)]
         lib.moe_w4_matvec.argtypes = [P, P, P, I32, I32, I32, I32, I32, I32, I32, I32, I32, P, P, U64, P]
         for name in EXPORTS:

@@ -348,14 +348,50 @@ __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((u
 // The tiles of a task that a group of warps has: [own_first(m, group), own_first(m, group + 1)).
 __device__ __forceinline__ int own_first(int m, int group) { return m * group / kGroupsM; }
 
-// mbar_wait_bounded, with the clock left alone until a thousand polls have failed: reading it takes
-// longer than most waits here.
-__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+// The ring between the copying warp and the warps that multiply.  Waits are bounded; when one gives up, no
+// copy may be issued into a slot whose last one has not landed, and none may be under way when the CTA
+// ends, since the shared memory is another CTA's then.  So a warp frees only slots that it has seen full
+// (a slot counts as freed when all have), and the copying warp, whichever way its loop ended, leaves when what
+// it has issued has landed.
+template <unsigned long long LIMIT_NS>
+struct Ring {
+  uint64_t* full;             // [stages], one arrival (the copying warp's) and the bytes
+  uint64_t* empty;            // [stages], kConsumers arrivals
+  volatile int* abort_flag;   // set by the first wait that gives up
+  int stages;
+
+  // mbar_wait_bounded, with the clock left alone until a thousand polls have failed: reading it takes
+  // longer than most waits here.
+  static __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* flag) {
 #pragma unroll 1
-  for (int i = 0; i < 1024; ++i)
-    if (mbar_try_wait(bar, parity)) return true;
-  return mbar_wait_bounded(bar, parity, abort_flag);
-}
+    for (int i = 0; i < 1024; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    return mbar_wait_bounded(bar, parity, flag, LIMIT_NS);
+  }
+  // Whole warps.  Has the slot's next stage come?
+  __device__ __forceinline__ bool take(int slot, uint32_t parity) const {
+    return __all_sync(0xffffffffu, wait_for(&full[slot], parity, abort_flag));
+  }
+  // The warp is done with a slot; `taken` is what take said of it.
+  __device__ __forceinline__ void free_slot(int slot, bool taken) const {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0 && taken) mbar_arrive(&empty[slot]);
+  }
+  // The copying warp: may the slot be filled again?
+  __device__ __forceinline__ bool reserve(int slot, uint32_t parity) const {
+    return __all_sync(0xffffffffu, wait_for(&empty[slot], parity, abort_flag) && !*abort_flag);
+  }
+  // The copying warp, at its end: have all of its `issued` stages landed?  The waits share one limit.
+  __device__ __forceinline__ bool drain(int issued) const {
+    bool landed = true;
+    if ((threadIdx.x & 31) == 0) {
+      volatile int gave_up = 0;
+      for (int i = issued > stages ? issued - stages : 0; i < issued; ++i)
+        landed &= wait_for(&full[i % stages], (uint32_t)(i / stages) & 1u, &gave_up);
+    }
+    return __all_sync(0xffffffffu, landed);
+  }
+};
 
 // One step of a warp: M records of 128 columns, `m_stride` bytes apart, times NT * 8 rows of x.  The
 // records are worked on side by side, so that M * NT chains of products are under way.
@@ -537,6 +573,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
   const int weights_bytes = tasks.most() * kSplit * kRecord, stage_bytes = weights_bytes + s_most_rows * kRowPiece;
   const int fit = (int)(kSmem - kSumBytes) / (stage_bytes > 0 ? stage_bytes : 1);
   const int stages = fit < kMaxStages ? fit : kMaxStages;
+  const Ring<kWaitLimitNs> ring = {s_full, s_empty, &s_abort, stages};
 
   if (warp >= kConsumers) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
@@ -602,22 +639,15 @@ __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
     uint32_t parity = issued == stages ? 0 : 1;    // a fresh slot counts as freed
     bool ok = true;
     for (; w.m; ++issued) {
-      ok = __all_sync(0xffffffffu, wait_for(&s_empty[slot], parity, &s_abort));
+      ok = ring.reserve(slot, parity);
       if (!ok) break;
       copy_weights(w, src, stage, slot);
       copy_rows(w, stage, slot);
       if (step_on(w, stage)) src = source_of(w);
       if (++slot == stages) { slot = 0; parity ^= 1; }
     }
-    if (!ok) {                                     // let the copies that are under way land
-      if (lane == 0) {
-        raise_error(&g_w4_error, kDevTimeoutProducer);
-        volatile int none = 0;
-        for (int i = issued > stages ? issued - stages : 0; i < issued; ++i)
-          wait_for(&s_full[i % stages], (uint32_t)(i / stages) & 1u, &none);
-      }
-      __syncwarp();
-    }
+    ok &= ring.drain(issued);
+    if (!ok && lane == 0) raise_error(&g_w4_error, kDevTimeoutProducer);
     return;
   }
 
@@ -646,7 +676,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
         for (int i = 0; i < 4; ++i) sums[m][nt][i] = 0.f;
 #pragma unroll 1
     for (int stage = 0; stage < p.stages; ++stage) {
-      if (ok) ok = __all_sync(0xffffffffu, wait_for(&s_full[slot], parity, &s_abort));
+      if (ok) ok = ring.take(slot, parity);
       const uint8_t* at = s_mem + slot * stage_bytes;
       const int left = p.k_steps - stage * kSplit, stride = (left < kSplit ? left : kSplit) * kRecord;
       if (ok && kw < left && (!turns || stage % kGroupsM == mg)) {
@@ -657,8 +687,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
         else if (kM > 2 && m_here == 2) multiply<T, NT, 2, G, ZEROS>(records, stride, x, kw, sums);
         else if (kM > 3 && m_here == 3) multiply<T, NT, 3, G, ZEROS>(records, stride, x, kw, sums);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s_empty[slot]);
+      ring.free_slot(slot, ok);
       if (++slot == stages) { slot = 0; parity ^= 1; }
     }
     // The sums of the warps that share tiles (a group, or all when they take turns) meet in shared
@@ -718,6 +747,72 @@ __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
       if (p.out_f32) static_cast<float*>(p.y)[r * p.N + n] = 0.f;
       else static_cast<T*>(p.y)[r * p.N + n] = from_float<T>(0.f);
     }
+  }
+}
+
+// Self-test of the ring's failure path: the product's ring with a wait limit of 2 ms, four slots of 1 KB and
+// `issues` stages, of which the copying warp issues all copies but number `missing`, so that the waits for
+// that one run out.  report: [0] stages issued, [1] the fewest stages that a multiplying warp took, [2] wrong words
+// in what was taken, [3] whether reserve ran out, [4] whether drain found a copy missing, [5] how many of the
+// last four stages had landed when the copying warp left.
+constexpr int kTestSlots = 4, kTestBytes = 1024;
+__global__ void __launch_bounds__((kConsumers + 1) * 32)
+w4_selftest_ring_kernel(const uint32_t* __restrict__ src, int issues, int missing, int* __restrict__ report) {
+  __shared__ __align__(128) uint32_t s_slots[kTestSlots][kTestBytes / 4];
+  __shared__ __align__(8) uint64_t s_full[kTestSlots], s_empty[kTestSlots];
+  __shared__ volatile int s_abort;
+  __shared__ int s_taken, s_wrong;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Ring<2000000> ring = {s_full, s_empty, &s_abort, kTestSlots};
+  if (threadIdx.x < kTestSlots) {
+    mbar_init(&s_full[threadIdx.x], 1);
+    mbar_init(&s_empty[threadIdx.x], kConsumers);
+    fence_mbar_init();
+  }
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    s_taken = issues;
+    s_wrong = 0;
+  }
+  __syncthreads();
+  if (warp == kConsumers) {
+    bool ok = true;
+    int issued = 0;
+    for (; issued < issues; ++issued) {
+      const int slot = issued % kTestSlots;
+      ok = ring.reserve(slot, (uint32_t)(issued / kTestSlots + 1) & 1u);
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&s_full[slot], kTestBytes);
+        if (issued != missing) bulk_copy(smem_u32(s_slots[slot]), src + issued * (kTestBytes / 4), kTestBytes, &s_full[slot]);
+      }
+      __syncwarp();
+    }
+    const bool landed = ring.drain(issued);
+    if (lane == 0) {
+      int there = 0;
+      for (int i = issued > kTestSlots ? issued - kTestSlots : 0; i < issued; ++i)
+        there += mbar_try_wait(&s_full[i % kTestSlots], (uint32_t)(i / kTestSlots) & 1u);
+      report[0] = issued;
+      report[3] = !ok;
+      report[4] = !landed;
+      report[5] = there;
+    }
+  } else {
+    bool ok = true;
+    for (int i = 0; i < issues; ++i) {
+      const int slot = i % kTestSlots;
+      if (ok && !(ok = ring.take(slot, (uint32_t)(i / kTestSlots) & 1u)) && lane == 0) atomicMin(&s_taken, i);
+      if (ok)
+        for (int k = lane; k < kTestBytes / 4; k += 32)
+          if (s_slots[slot][k] != __ldg(src + i * (kTestBytes / 4) + k)) atomicAdd(&s_wrong, 1);
+      ring.free_slot(slot, ok);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    report[1] = s_taken;
+    report[2] = s_wrong;
   }
 }
 
@@ -831,6 +926,16 @@ MOE_API int moe_w4_matvec(const void* x, const void* layout, const int32_t* offs
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return dtype == MOE_BF16 ? run_w4<__nv_bfloat16>(p, x, d, group_size, with_zeros != 0, sms, s)
                            : run_w4<__half>(p, x, d, group_size, with_zeros != 0, sms, s);
+}
+
+MOE_API int moe_w4_selftest_ring(const void* src, int32_t issues, int32_t missing, int32_t* report, void* stream) {
+  if (!src || !report || issues < 0 || issues > 4096 || missing < 0) return MOE_ERR_INVALID_ARGUMENT;
+  if (!aligned_to(src, 16) || !aligned_to(report, 4)) return MOE_ERR_MISALIGNED;
+  const int st = require_device(nullptr);
+  if (st != MOE_OK) return st;
+  w4_selftest_ring_kernel<<<1, (kConsumers + 1) * 32, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint32_t*>(src), issues, missing, report);
+  return cuda_status(cudaGetLastError());
 }
 
 MOE_API int moe_w4_read_device_error(void* stream, int32_t* device_error) {
