@@ -36,6 +36,7 @@
 //   the record's scales [8][128 / G][2] (for row g of the first 8: group by group, row g's and
 //   row g + 8's together), then, if there are any, its zero points likewise: a lane's
 //   share of them is together.
+#include <mutex>
 #include <type_traits>
 
 #include "rows.cuh"
@@ -81,8 +82,10 @@ struct W4Params {
   int out_f32, zero_rest;
 };
 
-// Set when a wait gave up; read and cleared by moe_w4_read_device_error.
-__device__ int g_w4_error;
+// Set when a wait gave up; taken by moe_w4_read_device_error: in one step, so that no error which is raised
+// meanwhile on another stream is cleared unread.
+__device__ int g_w4_error, g_w4_taken;
+__global__ void w4_take_error_kernel() { g_w4_taken = atomicExch(&g_w4_error, 0); }
 
 // --------------------------------------------------------------------------
 // The layout: a thread makes 16 bytes.  Padding (rows behind N, columns behind D) is
@@ -750,7 +753,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
   }
 }
 
-// Self-test of the ring's failure path: the product's ring with a wait limit of 2 ms, four slots of 1 KB and
+// Self-test of the ring's failure path: the product's ring with waits of a few ms, four slots of 1 KB and
 // `issues` stages, of which the copying warp issues all copies but number `missing`, so that the waits for
 // that one run out.  report: [0] stages issued, [1] the fewest stages that a multiplying warp took, [2] wrong words
 // in what was taken, [3] whether reserve ran out, [4] whether drain found a copy missing, [5] how many of the
@@ -813,6 +816,7 @@ w4_selftest_ring_kernel(const uint32_t* __restrict__ src, int issues, int missin
   if (threadIdx.x == 0) {
     report[1] = s_taken;
     report[2] = s_wrong;
+    if (s_taken < issues) raise_error(&g_w4_error, kDevTimeoutMma);
   }
 }
 
@@ -943,10 +947,12 @@ MOE_API int moe_w4_read_device_error(void* stream, int32_t* device_error) {
   const int st = require_device(nullptr);
   if (st != MOE_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  static std::mutex one_reader;                    // g_w4_taken is its own until it has been copied
+  std::lock_guard<std::mutex> lock(one_reader);
   int32_t v = 0;
-  const int32_t none = 0;
-  cudaError_t e = cudaMemcpyFromSymbolAsync(&v, g_w4_error, 4, 0, cudaMemcpyDeviceToHost, s);
-  if (e == cudaSuccess) e = cudaMemcpyToSymbolAsync(g_w4_error, &none, 4, 0, cudaMemcpyHostToDevice, s);
+  w4_take_error_kernel<<<1, 1, 0, s>>>();
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbolAsync(&v, g_w4_taken, 4, 0, cudaMemcpyDeviceToHost, s);
   if (e == cudaSuccess) e = cudaStreamSynchronize(s);
   if (e != cudaSuccess) return cuda_status(e);
   *device_error = v;

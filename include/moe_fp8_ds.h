@@ -346,16 +346,18 @@ MOE_API int moe_w4_matvec(const void* x, const void* layout, const int32_t* offs
                           int32_t dtype, int32_t out_dtype, int32_t zero_other_rows, void* y, void* workspace,
                           uint64_t workspace_bytes, void* stream);
 
-/* Failure-detection self-test of moe_w4_matvec's ring of copies, with waits of 2 ms: `issues` stages of
+/* Failure-detection self-test of moe_w4_matvec's ring of copies, with waits of a few ms: `issues` stages of
  * 1 KB from src (16-byte aligned) pass through four slots, all of them copied but number `missing` (issues or
  * more: none), so that the waits for that one run out.  report int32 [6]: stages issued, the fewest stages that
  * a multiplying warp took, wrong words in what was taken, whether the copying warp's wait for a slot ran out,
- * whether it left without all of its copies, how many of the last four stages had landed when it left.  */
+ * whether it left without all of its copies, how many of the last four stages had landed when it left.  Where a
+ * wait ran out, moe_w4_matvec's error word is set.                            */
 MOE_API int moe_w4_selftest_ring(const void* src, int32_t issues, int32_t missing, int32_t* report, void* stream);
 
-/* Synchronises `stream`, reads and clears the current device's error code of
+/* Synchronises `stream`, takes (reads and clears in one step) the current device's error code of
  * moe_w4_matvec: 0, or what a bounded wait that gave up left (the outputs of that call
- * are then not to be used).                                                  */
+ * are then not to be used).  One code stands for the device's streams; a call on another
+ * stream is covered once that stream's work is complete.                     */
 MOE_API int moe_w4_read_device_error(void* stream, int32_t* device_error);
 
 #ifdef __cplusplus
