@@ -87,6 +87,17 @@ struct W4Params {
 __device__ int g_w4_error, g_w4_taken;
 __global__ void w4_take_error_kernel() { g_w4_taken = atomicExch(&g_w4_error, 0); }
 
+// Whether this process has launched products on the current device: else its word is 0, and reading it needs
+// neither a stream nor a device of the right kind.
+std::atomic<bool> g_w4_launched[kMaxCachedDevices];
+bool w4_launched(bool now) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return now;
+  if (dev < 0 || dev >= kMaxCachedDevices) return true;
+  if (now) g_w4_launched[dev].store(true, std::memory_order_release);
+  return g_w4_launched[dev].load(std::memory_order_acquire);
+}
+
 // --------------------------------------------------------------------------
 // The layout: a thread makes 16 bytes.  Padding (rows behind N, columns behind D) is
 // zero.
@@ -830,6 +841,7 @@ int launch_w4(const W4Params& p, const void* x, int d, int sms, cudaStream_t s) 
                 "two stages");
   static std::atomic<void*> seen[kMaxCachedDevices];
   cudaError_t e = once_per_context(seen, [] {
+    w4_launched(true);
     return cudaFuncSetAttribute(w4_kernel<T, G, ZEROS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
   });
   if (e != cudaSuccess) return cuda_status(e);
@@ -937,6 +949,7 @@ MOE_API int moe_w4_selftest_ring(const void* src, int32_t issues, int32_t missin
   if (!aligned_to(src, 16) || !aligned_to(report, 4)) return MOE_ERR_MISALIGNED;
   const int st = require_device(nullptr);
   if (st != MOE_OK) return st;
+  w4_launched(true);
   w4_selftest_ring_kernel<<<1, (kConsumers + 1) * 32, 0, static_cast<cudaStream_t>(stream)>>>(
       static_cast<const uint32_t*>(src), issues, missing, report);
   return cuda_status(cudaGetLastError());
@@ -944,8 +957,8 @@ MOE_API int moe_w4_selftest_ring(const void* src, int32_t issues, int32_t missin
 
 MOE_API int moe_w4_read_device_error(void* stream, int32_t* device_error) {
   if (!device_error) return MOE_ERR_INVALID_ARGUMENT;
-  const int st = require_device(nullptr);
-  if (st != MOE_OK) return st;
+  *device_error = 0;
+  if (!w4_launched(false)) return MOE_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   static std::mutex one_reader;                    // g_w4_taken is its own until it has been copied
   std::lock_guard<std::mutex> lock(one_reader);

@@ -218,8 +218,8 @@ def read_device_error(device: torch.device | None = None) -> int:
     error happened since the last read.  The reads run on the current stream after it has
     waited on each workspace's last-use event, so streams the caller has destroyed since
     are never touched.  The 4-bit products' error word (one for the device) is taken with
-    them, after the current stream's earlier work; products on other streams are covered
-    once their streams' work is complete."""
+    them where this process has made such products, after the current stream's earlier
+    work; products on other streams are covered once their streams' work is complete."""
     lib = _lib.load()
     idx = _device_index(device)
     with _ws_lock:

@@ -357,7 +357,8 @@ MOE_API int moe_w4_selftest_ring(const void* src, int32_t issues, int32_t missin
 /* Synchronises `stream`, takes (reads and clears in one step) the current device's error code of
  * moe_w4_matvec: 0, or what a bounded wait that gave up left (the outputs of that call
  * are then not to be used).  One code stands for the device's streams; a call on another
- * stream is covered once that stream's work is complete.                     */
+ * stream is covered once that stream's work is complete.  Where this process has launched
+ * no such call on the device, the code is 0 and `stream` is left alone.      */
 MOE_API int moe_w4_read_device_error(void* stream, int32_t* device_error);
 
 #ifdef __cplusplus
