@@ -12,6 +12,8 @@
 // elements + 2 bytes (forward), 1 + 2 elements + 2 bytes (backward) for each
 // column, so the kept codes cost the backward pass half of the reads that kept
 // 16-bit inputs would.
+#include <type_traits>
+
 #include "rows.cuh"
 
 namespace moe {
@@ -22,11 +24,22 @@ constexpr int kElems = kBlock / kLanes;          // 8 columns a thread
 constexpr int kThreads = 256;
 constexpr int kRowsAtOnce = kThreads / kLanes;   // rows of a CTA in one step
 
-// sigmoid in fp32.  16-bit outputs keep 11 bits at most, so the short forms
-// (about 2^-21 off) cost them nothing; fp32 outputs get the full ones.
-template <typename T>
+// sigmoid in fp32, 1 / (1 + exp(-v)), down to the least fp32 number: from v = -88 on exp(-v) leaves fp32, while
+// up * v * sigmoid(v) is a number that bf16 and fp32 hold.  16-bit outputs keep 11 bits at most, so they take the
+// hardware's approximations of 2^x and 1 / d, with t = exp(-v / 2) and the sum 2^24 times smaller, which nothing
+// overflows where the result is not 0: 2^-24 / (2^-24 + 2^-24 t t).  It is off by less than 5 + 1.173 |v|
+// units of 2^-23.  fp32 outputs get the full exp and division; below -kFar their sigmoid is exp(v) itself (FAR:
+// a block's gates may be there).
+constexpr float kFar = 80.f;
+template <typename T, bool FAR>
 __device__ __forceinline__ float sigmoid(float v) {
-  if constexpr (sizeof(T) == 2) return __fdividef(1.f, 1.f + __expf(-v));
+  if constexpr (sizeof(T) == 2) {
+    float t, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(v * -0.72134752f));   // log2(e) / 2
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(t * 0x1p-24f, t, 0x1p-24f)));
+    return r * 0x1p-24f;
+  }
+  if (FAR && v < -kFar) return expf(v);
   return 1.f / (1.f + expf(-v));
 }
 
@@ -138,10 +151,11 @@ __device__ __forceinline__ void store_codes(uint8_t* q, int lane, int width, con
   }
 }
 
-// Codes of a block and its scale (the same in all 16 lanes).
+// Codes of a block and its scale (the same in all 16 lanes); `bits` becomes the largest magnitude's.
 template <typename T, int N>
-__device__ __forceinline__ float keep_block(uint8_t* q, int lane, int width, const Piece<T, N>& x, const float (&v)[kElems]) {
-  uint32_t bits = largest<T, N>(x, v);
+__device__ __forceinline__ float keep_block(uint8_t* q, int lane, int width, const Piece<T, N>& x, const float (&v)[kElems],
+                                            uint32_t& bits) {
+  bits = largest<T, N>(x, v);
 #pragma unroll
   for (int off = kLanes / 2; off; off >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, off));
   float s = __fdiv_rn(__uint_as_float(bits), kFp8Max);
@@ -176,7 +190,7 @@ __device__ __forceinline__ void kept_values(const Piece<uint8_t, N>& q, float s,
 // block, [2 * blocks][R]) are written as whole lines; neighbouring CTAs take
 // neighbouring blocks.  U rows are in flight in each thread.
 template <typename T, int N, int U, bool KEEP>
-__global__ void __launch_bounds__(kThreads, KEEP ? 5 : 1)   // 32768 x 4096 bf16, kept: 117 us, unbounded 127 us
+__global__ void __launch_bounds__(kThreads, 5)   // 32768 x 4096 fp16: 63 us, unbounded 66
 swiglu_kernel(const T* __restrict__ x, int R, int I, int blocks, T* __restrict__ y, uint8_t* __restrict__ q,
               float* __restrict__ scale) {
   griddep_wait();
@@ -201,16 +215,28 @@ swiglu_kernel(const T* __restrict__ x, int R, int I, int blocks, T* __restrict__
     float up[kElems], gate[kElems], out[kElems];
     to_floats<T, N>(up_in[u], up);
     to_floats<T, N>(gate_in[u], gate);
+    uint32_t bits = 0;                             // of the block's largest gate
     if constexpr (KEEP) {
       uint8_t* p = q + (size_t)r * 2 * I + col;
-      const float su = keep_block<T, N>(p, lane, w, up_in[u], up), sg = keep_block<T, N>(p + I, lane, w, gate_in[u], gate);
+      const float su = keep_block<T, N>(p, lane, w, up_in[u], up, bits), sg = keep_block<T, N>(p + I, lane, w, gate_in[u], gate, bits);
       if (lane == 0 && r < R) {
         scale[(size_t)b * R + r] = su;
         scale[(size_t)(blocks + b) * R + r] = sg;
       }
     }
+    bool far = false;                              // a thread's gates, or the block's where they were compared
+    if constexpr (sizeof(T) == 4) {
+      far = bits > __float_as_uint(kFar);
 #pragma unroll
-    for (int i = 0; i < kElems; ++i) out[i] = gate[i] * sigmoid<T>(gate[i]) * up[i];
+      for (int i = 0; i < kElems; ++i) far |= !KEEP && gate[i] < -kFar;
+    }
+    if (!far) {
+#pragma unroll
+      for (int i = 0; i < kElems; ++i) out[i] = gate[i] * sigmoid<T, false>(gate[i]) * up[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kElems; ++i) out[i] = gate[i] * sigmoid<T, true>(gate[i]) * up[i];
+    }
     store_piece<T, N>(y + (size_t)r * I + col, lane, w, out);
   }
 }
@@ -247,12 +273,16 @@ swiglu_backward_kernel(const T* __restrict__ g, const uint8_t* __restrict__ q, c
     kept_values<N>(up_in[u], su[u], up);
     kept_values<N>(gate_in[u], sg[u], gate);
     to_floats<T, N>(dy_in[u], dy);
+    auto gradients = [&](auto far) {
 #pragma unroll
-    for (int i = 0; i < kElems; ++i) {
-      const float sig = sigmoid<T>(gate[i]), gs = dy[i] * sig;
-      du[i] = gs * gate[i];
-      dg[i] = gs * up[i] * (1.f + gate[i] * (1.f - sig));
-    }
+      for (int i = 0; i < kElems; ++i) {
+        const float sig = sigmoid<T, decltype(far)::value>(gate[i]), gs = dy[i] * sig;
+        du[i] = gs * gate[i];
+        dg[i] = gs * up[i] * (1.f + gate[i] * (1.f - sig));
+      }
+    };
+    if (sizeof(T) == 2 || sg[u] < kFar / kFp8Max) gradients(std::false_type{});   // the block's largest gate is 448 times its scale
+    else gradients(std::true_type{});
     T* p = grad_x + (size_t)r * 2 * I + col;
     store_piece<T, N>(p, lane, w, du);
     store_piece<T, N>(p + I, lane, w, dg);
@@ -287,16 +317,17 @@ int run_backward_u(const void* dy, const void* q, const float* scale, int R, int
 }
 
 // Rows in flight in a thread: two where that still makes 8 CTAs for each SM and a thread's accesses
-// are of 16 bytes.  (us for the forward pass / the one that keeps codes / the backward
-// pass, two rows and one: 32768 x 4096 bf16 70 / 119 / 98 and 80 / 123 / 109; 512 x 4096 bf16
-// 8.2 / 10.2 / 8.2 and 8.2 / 8.2 / 8.2; single columns, 32768 x 2002 bf16, 51 / 96 / 90 and
-// 51 / 86 / 82; four, 32768 x 2008 bf16, 47 / 64 / 55 and 39 / 68 / 55.)
+// are of 16 bytes, or in the forward passes of 4 columns.  (us for the forward pass / the one that keeps codes / the
+// backward pass, two rows and one: 32768 x 4096 bf16 62 / 111 / 94 and 73 / 117 / 100, fp16 63 / 109 / 103 and 67 /
+// 115 / 99; 16384 x 4096 fp32 61 / 81 / 73 and 60 / 81 / 83, 16384 x 2004 fp32 30 / 50 / 44 and 30 / 46 / 43; 512 x 4096 bf16 4.5 / 4.6 / 4.6 either way; four
+// columns at a time, 32768 x 2008 bf16, 35 / 62 / 53 and 37 / 63 / 51; single ones, 32768 x 2002 bf16, 43 / 100 / 86
+// and 45 / 84 / 71.)
 constexpr int kFlight = 2;
 bool many_rows(int R, int I) { return swiglu_grid(R, I, kFlight).ctas >= 148 * 8; }
 
 template <typename T, int N>
 int run_forward(const void* x, int R, int I, void* y, void* q, float* scale, cudaStream_t s) {
-  if constexpr (N * sizeof(T) >= 16)
+  if constexpr (N >= 4)
     if (many_rows(R, I)) return run_forward_u<T, N, kFlight>(x, R, I, y, q, scale, s);
   return run_forward_u<T, N, 1>(x, R, I, y, q, scale, s);
 }
