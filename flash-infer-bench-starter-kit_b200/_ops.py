@@ -7,6 +7,7 @@ from __future__ import annotations
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _lib
 
@@ -47,6 +48,15 @@ def check_tensor(name, t, dtypes, shape, device):
         raise ValueError(f"{name} is on {t.device}, expected {device}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
+
+
+def check_output(name, t):
+    """A tensor that a call overwrites: autograd is told, so that a backward pass which saved its values
+    raises, as after any operation in place."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient that writing into it would not give: detach it")
+    if not t.is_inference():
+        increment_version(t)
 
 
 def differentiable_once(backward):

@@ -20,7 +20,7 @@ import functools
 import torch
 
 from . import _lib
-from ._ops import DTYPES, INT32_MAX, call, check_tensor, refuse_tangent
+from ._ops import DTYPES, INT32_MAX, call, check_output, check_tensor, refuse_tangent
 from .activation import swiglu
 from .tokens import _combine, dispatch, sort_tokens
 
@@ -144,6 +144,7 @@ def w4_matvec(x: torch.Tensor, weights: W4Weights, offsets: torch.Tensor | None 
         out = torch.empty(R, weights.n, dtype=out_dtype, device=dev)
     else:
         check_tensor("out", out, (x.dtype, torch.float32) if out_dtype is None else (out_dtype,), (R, weights.n), dev)
+        check_output("out", out)
     if x.data_ptr() % 16:
         x = x.clone()
     need = _workspace_bytes(R, weights.d)
@@ -173,6 +174,7 @@ def moe_w4(hidden_states: torch.Tensor, topk_ids: torch.Tensor, topk_weights: to
     check_tensor("hidden_states", hidden_states, (w13.dtype,), (T, w13.d), topk_ids.device)
     if output is not None:
         check_tensor("output", output, (hidden_states.dtype,), (T, w2.n), topk_ids.device)
+        check_output("output", output)
     rows = w4_matvec(dispatch(hidden_states, order), w13, order.offsets)
     # fp32 from the second product to the sum over k: one rounding, as in the fused layer
     down = w4_matvec(swiglu(rows), w2, order.offsets, out_dtype=torch.float32)
