@@ -4,6 +4,8 @@ on the tensors' device and its current stream."""
 
 from __future__ import annotations
 
+import types
+
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
@@ -22,11 +24,15 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+# The level of forward-mode differentiation that is open, -1 for none: torch's own variable where there is
+# one (unpack_dual, which would tell as well, takes 0.7 us a tensor), else asked for each tensor.
+_dual_level = forward_ad if hasattr(forward_ad, "_current_level") else types.SimpleNamespace(_current_level=0)
+
+
 def refuse_tangent(name, t):
     """Refuse a dual tensor of forward-mode differentiation.  It need not require a gradient, so no
-    ``autograd.Function`` would see it, and its tangent would be lost without a word.  ``unpack_dual``
-    takes 0.7 us, so it is asked only while a dual level is open."""
-    if getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+    ``autograd.Function`` would see it, and its tangent would be lost without a word."""
+    if _dual_level._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
         raise ValueError(f"{name} carries a tangent: there is no forward-mode derivative")
 
 
@@ -41,7 +47,8 @@ def check_tensor(name, t, dtypes, shape, device):
     if len(got) != len(shape) or any((n != -1 and n != m) or m > INT32_MAX for n, m in zip(shape, got)):
         want = ", ".join(f"at most {INT32_MAX}" if n == -1 else str(n) for n in shape)
         raise ValueError(f"{name} has shape {tuple(got)}, expected ({want})")
-    refuse_tangent(name, t)
+    if _dual_level._current_level >= 0:
+        refuse_tangent(name, t)
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor (no CPU path)")
     if device is not None and t.get_device() != device.index:
