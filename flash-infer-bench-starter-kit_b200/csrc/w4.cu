@@ -12,8 +12,9 @@
 // -zero * (sum of x over the group), made once for each row of x, and is scaled in
 // fp32; the factors 2^24 and 1/16 are left to the last step, and only the output is
 // rounded.
-// What else was built and measured (us; 8 matrices of 4096 x 7168 times a row each /
-// 32 of them times 16 rows; this form 38 / 138): zero points subtracted from the operands, 16 more
+// What else was built and measured (us, caches flushed before a call; 8 matrices of
+// 4096 x 7168 times a row each / 32 of them times 16 rows; this form 37 / 139, and 30 /
+// 131 call after call on weights from memory): zero points subtracted from the operands, 16 more
 // instructions for each 16 x 64 codes, 40 / 208; e4m3 operands, where a byte 0..15 is
 // q * 2^-9, 55 / 428 (four times the executed instructions); tcgen05.mma with the decoded weights in tensor memory, 112 / 410 (8
 // products of N = 16 and their hand-overs took 2000 clocks for 128 x 128 codes that
@@ -58,8 +59,8 @@ constexpr int kFewRegisters = 40, kManyRegisters = 232;
 constexpr int kMaxStages = 16;            // of the ring, as many as fit
 constexpr int kEarly = 4;                 // stages whose weights are copied before the rows of x are there
 // Rows of x in a task.  Four products of 8 rows side by side fit the registers except with
-// groups of 32, where they spill: 25 to 32 rows of all of 32 experts 264 us, in two tasks
-// 230 us (groups of 128: 211 and 267 us).
+// groups of 32, where they spill: 32 rows of all of 32 experts of 7168 x 2048 217 us, in two
+// tasks 195 us (4096 x 7168 in groups of 128: 211 and, in two tasks, 267 us).
 __host__ __device__ constexpr int max_rows(int G) { return G == 32 ? 24 : 32; }
 constexpr int kMaxExperts = 1024;
 constexpr int kStageK = kSplit * kStepK;  // columns of a stage
@@ -350,10 +351,10 @@ struct Tasks {
     size_task(w);
   }
 };
-// What a tile costs with this many rows of x, in sixths of the cost with 8: measured with all of 32
-// experts at 8, 16, 24 and 32 rows less 10 us of start (4096 x 7168, groups of 128: 98, 124, 159 and
-// 198 us; 7168 x 2048, groups of 32: 75, 112 and 151 us, 25 to 32 rows being two chunks).  512 rows over
-// the 32 experts as a router leaves them: 175 us with 6, 8, 11, 14 here, 165 us with these.
+// What a tile costs with this many rows of x, in sixths of the cost with 8.  All of 32 experts with 8, 16, 24 and
+// 32 rows take, call after call, 93, 131, 167 and 202 us (4096 x 7168, groups of 128), 96, 137 and 177 us (groups
+// of 64, which go by the same costs) and 71, 103 and 148 us (7168 x 2048, groups of 32; 25 to 32 rows are two chunks).
+// 512 rows over the 32 experts as a router leaves them: 175 us with 6, 8, 11, 14 here, 165 us with these.
 template <int G>
 __device__ __forceinline__ int chunk_cost(int rows) {
   return rows <= 8 ? 6 : rows <= 16 ? (G == 32 ? 9 : 8) : rows <= 24 ? (G == 32 ? 12 : 10) : 12;
@@ -365,8 +366,10 @@ __device__ __forceinline__ int own_first(int m, int group) { return m * group / 
 // The ring between the copying warp and the warps that multiply.  Waits are bounded; when one gives up, no
 // copy may be issued into a slot whose last one has not landed, and none may be under way when the CTA
 // ends, since the shared memory is another CTA's then.  So a warp frees only slots that it has seen full
-// (a slot counts as freed when all have), and the copying warp, whichever way its loop ended, leaves when what
-// it has issued has landed.
+// (a slot counts as freed when all have), and the copying warp, whichever way its loop ended, stays until the
+// others are through with all stages, or else until what it has issued has landed.  (It stays at a barrier:
+// polling the stages instead, beside warps that multiply, took a row times 4096 x 7168 from 11.0 to 13.2 us.)
+constexpr int kRingBarrier = 4;           // of the named barriers
 template <unsigned long long LIMIT_NS>
 struct Ring {
   uint64_t* full;             // [stages], one arrival (the copying warp's) and the bytes
@@ -393,10 +396,19 @@ struct Ring {
   }
   // The copying warp: may the slot be filled again?
   __device__ __forceinline__ bool reserve(int slot, uint32_t parity) const {
-    return __all_sync(0xffffffffu, wait_for(&empty[slot], parity, abort_flag) && !*abort_flag);
+    return __all_sync(0xffffffffu, wait_for(&empty[slot], parity, abort_flag));
   }
-  // The copying warp, at its end: have all of its `issued` stages landed?  The waits share one limit.
+  // A multiplying warp, after its last stage, taken or not.
+  __device__ __forceinline__ void leave() const {
+    __syncwarp();
+    asm volatile("bar.arrive %0, %1;" ::"n"(kRingBarrier), "n"((kConsumers + 1) * 32) : "memory");
+  }
+  // The copying warp, at its end: have all of its `issued` stages landed?  Where no wait gave up they have been
+  // taken; else the waits for them share one limit.
   __device__ __forceinline__ bool drain(int issued) const {
+    __syncwarp();
+    named_bar_sync(kRingBarrier, (kConsumers + 1) * 32);
+    if (!*abort_flag) return true;
     bool landed = true;
     if ((threadIdx.x & 31) == 0) {
       volatile int gave_up = 0;
@@ -509,8 +521,8 @@ __device__ __forceinline__ void multiply(const uint8_t* records, int m_stride, c
   }
 }
 
-// Measured, 32 experts of 4096 x 7168 in groups of 128, rows for each: 8 107 us (69% of the memory's
-// rate), 16 138, 24 173, 32 212.  Up to 8 rows memory and the copies' start bound it; beyond, the
+// Measured, 32 experts of 4096 x 7168 in groups of 128, rows for each, caches flushed before a call: 8 107 us
+// (69% of the memory's rate), 16 139, 24 176, 32 211; call after call 93 (79%), 131, 167, 202.  Up to 8 rows memory and the copies' start bound it; beyond, the
 // products do: an mma.sync holds a scheduler for 8 clocks (2.0 an SM, measured), and the 4 to 10 other
 // instructions that each comes with (5 of them decode 8 codes for all rows) hardly overlap with it.
 //
@@ -671,7 +683,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
   griddep_launch_dependents();
   const int kw = warp % kSplit, mg = warp / kSplit, g = lane >> 2, t = lane & 3;
   // With few tiles the groups of warps take turns at the stages instead of sharing out the tiles:
-  // one row of x and a matrix of 4096 x 7168, call after call, 13.9 -> 11.5 us.
+  // one row of x and a matrix of 4096 x 7168, replayed call after call, 12.3 -> 11.0 us, 32 rows and 2048 x 7168
+  // 17.3 -> 15.9 us.
   const bool turns = tasks.most() <= kM;
   const int parties = turns ? kConsumers * 32 : kSplit * 32;   // threads that add up the same sums
   int buffer = 0;
@@ -747,6 +760,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_kernel(const W4Params p) {
     else if (work.cnt <= 24) run(work, std::integral_constant<int, 3>{});
     else if constexpr (max_rows(G) > 24) run(work, std::integral_constant<int, 4>{});
   }
+  ring.leave();
   if (!ok && lane == 0) raise_error(&g_w4_error, kDevTimeoutMma);
   if (p.zero_rest && p.offsets) {                  // rows of no expert
     int a = __ldg(p.offsets), b = __ldg(p.offsets + p.E);
@@ -822,6 +836,7 @@ w4_selftest_ring_kernel(const uint32_t* __restrict__ src, int issues, int missin
           if (s_slots[slot][k] != __ldg(src + i * (kTestBytes / 4) + k)) atomicAdd(&s_wrong, 1);
       ring.free_slot(slot, ok);
     }
+    ring.leave();
   }
   __syncthreads();
   if (threadIdx.x == 0) {
