@@ -1,7 +1,9 @@
 """Expert products with 4-bit weights, for decoding.
 
-Reading the experts' weights bounds a decode step of the layer, so 4-bit
-weights with group scales halve what its FP8 experts read:
+Reading the experts' weights bounds a decode step of the layer, and 4-bit
+weights with group scales are half as many bytes as its FP8 experts (what that
+gives in time depends on the batch: with all of 256 experts here and 16 tokens
+``moe_w4`` takes 475 us and ``kernel(...)`` 516, with 64 tokens 1040 and 925):
 
     w13 = W4Weights(*quantize_w4(w, group_size=128), group_size=128)   # once: [E, N, D] weights
     y   = w4_matvec(rows, w13, order.offsets)     # rows sorted by expert (sort_tokens, dispatch)
@@ -63,7 +65,8 @@ class W4Weights:
 
     Column 2j of a row is the low half of its byte j.  A weight is ``(code - zero) * scale`` with
     ``scales`` [E, N, D / group_size] in fp16 or bf16, the type of the rows it will multiply, and
-    ``zeros`` uint8 of the same shape (0 to 15) or None for 8 everywhere."""
+    ``zeros`` uint8 of the same shape (0 to 15) or None for 8 everywhere.  Scales of magnitude 2^-100 to 2^100
+    keep all sums within fp32's normal numbers."""
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None, *,
                  group_size: int):
@@ -123,7 +126,8 @@ def w4_matvec(x: torch.Tensor, weights: W4Weights, offsets: torch.Tensor | None 
     single matrix.  Rows outside ``[offsets[0], offsets[E])`` are zero in a new result and left as they
     were in a given ``out``.  The weights of each expert with rows are read once for up to 32 rows, so
     this is the product for decode batches; prefill batches want a GEMM.  A row of ``x`` with an infinity or a
-    NaN has no finite products."""
+    NaN has no finite products.  Equal calls give equal bits; a row's last bits may differ between calls with
+    other rows beside it, since the order of its sums goes by the whole call's share for each SM."""
     if not isinstance(weights, W4Weights):
         raise TypeError("weights must be W4Weights")
     check_tensor("x", x, (weights.dtype,), (-1, weights.d), None)

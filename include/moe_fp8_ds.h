@@ -257,8 +257,9 @@ MOE_API int moe_fp8_ds_ep_combine(const void* partials, const int32_t* slot, int
  * Operators around the expert products (no counterpart in the reference, which
  * has these steps only inside its fused forward call).  Types are moe_dtype
  * values; tensors are contiguous and row-major; pointers are aligned to their
- * element (16-byte alignment gives the widest accesses).  No call keeps state or
- * needs a workspace.
+ * element (16-byte alignment gives the widest accesses).  No call keeps state but
+ * moe_w4_matvec, which sets an error word when a wait gives up and also is the only
+ * one that needs a workspace.
  * ------------------------------------------------------------------------- */
 typedef enum moe_dtype {
   MOE_F32 = 0,
@@ -338,7 +339,8 @@ MOE_API int moe_w4_lay_out(const void* codes, const void* scales, const void* ze
  * The rows go through the workspace (moe_w4_workspace_size bytes, 16-byte aligned, any
  * contents, not shared by calls that may overlap), bf16 ones scaled by a power of two
  * each into fp16: values more than 2^28 below the row's largest are off by at most
- * 2^-39 of that, others by nothing.  A row with an infinity or a NaN has no finite
+ * 2^-39 of that, others by nothing.  Scales of magnitude 2^-100 to 2^100 keep the sums
+ * within fp32's normal numbers.  A row with an infinity or a NaN has no finite
  * products.  x is 16-byte aligned.  E * ceil(R / 24) * max(n / 16, 16) < 2^31. */
 MOE_API int moe_w4_workspace_size(int32_t num_rows, int32_t d, uint64_t* bytes);
 MOE_API int moe_w4_matvec(const void* x, const void* layout, const int32_t* offsets, int32_t num_rows,
