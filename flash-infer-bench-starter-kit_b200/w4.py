@@ -170,6 +170,9 @@ def moe_w4(hidden_states: torch.Tensor, topk_ids: torch.Tensor, topk_weights: to
             raise TypeError(f"{name} must be W4Weights")
     if w13.num_experts != w2.num_experts or w13.n != 2 * w2.d:
         raise ValueError(f"w13 has {w13.num_experts} experts of {w13.n} rows, w2 {w2.num_experts} of {w2.d} columns")
+    for name, t in (("hidden_states", hidden_states), ("topk_weights", topk_weights)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
     if (hidden_states.requires_grad or topk_weights.requires_grad) and torch.is_grad_enabled():
         raise ValueError("moe_w4 has no gradient: detach its inputs or call it under torch.no_grad()")
     order = sort_tokens(topk_ids, w13.num_experts, local_expert_offset)
