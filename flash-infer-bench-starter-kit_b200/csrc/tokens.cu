@@ -322,9 +322,12 @@ combine_backward_kernel(const TOut* __restrict__ grad_out, const TRow* __restric
 // The two kernels above for rows of whole 16-byte pieces and at most 8 picks, where
 // bandwidth counts.  With the rows in registers a thread needs 100 to 180 of them and too
 // few threads fit to cover the memory's latency (4096 tokens x 8 x 7168 bf16: combine 127,
-// its gradients 215 us; with these 98 us, 5.4 TB/s, and 168 us, 5.9 TB/s).  Here every thread copies its own pieces of the next tokens
-// asynchronously into its own places in shared memory, kAhead steps ahead of the sums: no
-// registers, no barrier, and twice 256 threads x 2 steps x 128 bytes on their way on an SM.
+// its gradients 215 us; with these 84 us, 6.3 TB/s, and 161 us, 6.2 TB/s, call after call).  Here every
+// thread copies its own pieces of the next tokens asynchronously into its own places in
+// shared memory, two steps ahead of the sums: no registers, no barrier, and twice 256
+// threads x 2 steps x 128 bytes on their way on an SM.  More than 8 picks stay with the
+// kernels above (2048 tokens x 16 x 7168 bf16: 94 and 200 us, memory's floor 76 and 148;
+// 3640 x 9 x 7168, a second batch for one pick: 149 and 270, floor 80 and 151).
 // --------------------------------------------------------------------------
 constexpr int kStreamThreads = 256, kSteps = 3;   // places for 3 steps: 2 ahead
 
